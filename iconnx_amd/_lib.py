@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libiconnx_hip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "iconnx_hip.h")
 
-ICX_I8, ICX_U8, ICX_I32, ICX_F32, ICX_I64, ICX_BOOL = 0, 1, 2, 3, 4, 5
+ICX_I8, ICX_U8, ICX_I32, ICX_F32, ICX_I64, ICX_BOOL, ICX_F16, ICX_BF16 = 0, 1, 2, 3, 4, 5, 6, 7
 # status codes (include/iconnx_hip.h)
 ICX_OK, ICX_ERR_INVALID_ARG, ICX_ERR_SHAPE, ICX_ERR_DTYPE, ICX_ERR_WORKSPACE, ICX_ERR_HIP = 0, 1, 2, 3, 4, 5
 ICX_ERR_UNSUPPORTED, ICX_ERR_KERNEL = 6, 7
@@ -40,6 +40,22 @@ class OpProfile(ctypes.Structure):
                 ("gpu_us", ctypes.c_float), ("cpu_us", ctypes.c_float)]
 
 
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_size", ctypes.c_int32), ("bits", ctypes.c_int32)]
+
+
+class KvAttention(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("page_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p), ("q_starts", ctypes.c_void_p),
+                ("slopes", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("max_rows", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("window", ctypes.c_int32), ("causal", ctypes.c_int32)]
+
+
 class Chain(ctypes.Structure):
     _fields_ = [("n_ops", ctypes.c_int32), ("reserved", ctypes.c_int32),
                 ("ops", ChainOp * MAX_CHAIN)]
@@ -51,7 +67,7 @@ class Chain(ctypes.Structure):
 
 _lib = None
 
-P, S, I = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+P, S, I, LL = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64
 C, CP = ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p)
 SIGNATURES = {
     "icx_status_str": ([I], ctypes.c_char_p),
@@ -92,6 +108,16 @@ SIGNATURES = {
     "icx_transpose": ([P, P, S, I, P, P, P], I),
     "icx_matmul_f32": ([P, P, P, S, I, S, S, S, P], I),
     "icx_attention_f32": ([P, P, P, P, S, S, S, S, S, S, S, S, ctypes.c_float, I, I, P], I),
+    "icx_token_weight_bytes": ([S, S], S),
+    "icx_pack_token_weight": ([P, P, S, S, P], I),
+    "icx_quantize_tokens": ([P, P, I, S, S, LL, P, P], I),
+    "icx_token_qlinear_workspace_size": ([S, S, S, I], S),
+    "icx_token_qlinear": ([P, P, I, LL, P, S, S, S, P, P, P, P, I, LL, P, S], I),
+    "icx_kv_cache_bytes": ([P], S),
+    "icx_kv_cache_write": ([P, P, P, P, I, S, LL, LL, LL, LL, P, I], I),
+    "icx_kv_cache_read": ([P, P, P, I, S, P, P, I], I),
+    "icx_kv_cache_attention_workspace_size": ([P, P], S),
+    "icx_kv_cache_attention": ([P, P, P, P, S], I),
     "icx_graph_create": ([], P),
     "icx_graph_destroy": ([P], None),
     "icx_graph_add_input": ([P, C, I, P], I),

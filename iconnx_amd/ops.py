@@ -27,9 +27,9 @@ import struct
 import numpy as np
 import torch
 
-from ._lib import (BCAST_COL, BCAST_FULL, BCAST_ROW, BCAST_SCALAR, ICX_F32, ICX_I8, ICX_I32, ICX_I64,
-                   ICX_U8, MAX_CHAIN, OP_ADD, OP_DIV, OP_ERF, OP_MUL, OP_MUL_SAVED, OP_SAVE,
-                   OP_SUB, Chain, IconnxError, check, lib)
+from ._lib import (BCAST_COL, BCAST_FULL, BCAST_ROW, BCAST_SCALAR, ICX_BF16, ICX_F16, ICX_F32, ICX_I8, ICX_I32,
+                   ICX_I64, ICX_U8, MAX_CHAIN, OP_ADD, OP_DIV, OP_ERF, OP_MUL, OP_MUL_SAVED, OP_SAVE,
+                   OP_SUB, Chain, IconnxError, KvAttention, KvCacheDesc, check, lib)
 
 ERR_SHAPE, ERR_DTYPE, ERR_INVALID, ERR_UNSUPPORTED = 2, 3, 1, 6
 _DT = {torch.int8: ICX_I8, torch.uint8: ICX_U8, torch.int32: ICX_I32, torch.float32: ICX_F32}
@@ -573,6 +573,238 @@ def gpu_attention(q, k, v, heads, scale, scale_div=True, scale_q=False):
     check(lib().icx_attention_f32(_stream(), _p(q), _p(k), _p(v), B, S, heads, D, HD, HD, HD, HD,
                                   ctypes.c_float(scale), 1 if scale_div else 0,
                                   1 if scale_q else 0, _p(out)))
+    return out
+
+
+# ---------------------------------------------------------------------------------------
+# Decoder operators: products with a scale for each token, the quantized key / value cache
+# ---------------------------------------------------------------------------------------
+_FLOAT = {torch.float32: ICX_F32, torch.float16: ICX_F16, torch.bfloat16: ICX_BF16}
+_INDEX = {torch.int32: ICX_I32, torch.int64: ICX_I64}
+
+
+def _float_code(t, who):
+    code = _FLOAT.get(t.dtype if isinstance(t, torch.Tensor) else t)
+    if code is None:
+        raise IconnxError(ERR_DTYPE, "%s: dtype %s unsupported (must be Float32, Float16 or BFloat16)"
+                          % (who, _name(t.dtype if isinstance(t, torch.Tensor) else t)))
+    return code
+
+
+def _one_device(who, *ts):
+    """Every tensor on the current device: the kernels run there, on its current stream."""
+    _require_cuda(*ts)
+    here = _cur_device() if _cur_device else torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != here:
+            raise IconnxError(ERR_INVALID, "%s: a tensor is on device %d, the current one is %d" % (who, t.get_device(), here))
+
+
+def _rows(x):
+    """x [..., K] as rows: (rows, K, row stride, the tensor that holds them)."""
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x.shape[0], x.shape[1], x.stride(0), x
+    x = _dense(x)
+    K = x.shape[-1]
+    return (x.numel() // K if K else 0), K, K, x
+
+
+class TokenWeight:
+    """An int8 weight [K, N] with a float32 scale for each output channel [N], packed once for
+    :func:`gpu_token_qlinear`."""
+
+    def __init__(self, b, scale):
+        who = "TokenWeight"
+        if b.dtype != torch.int8:
+            raise IconnxError(ERR_DTYPE, "%s: the weight must be Int8, got %s" % (who, _name(b.dtype)))
+        if scale.dtype != _F32:
+            raise IconnxError(ERR_DTYPE, "%s: the scale must be Float32, got %s" % (who, _name(scale.dtype)))
+        if b.dim() != 2 or tuple(scale.shape) != (b.shape[1],):
+            raise IconnxError(ERR_SHAPE, "%s: a weight [K, N] and a scale [N] (got %s and %s)"
+                              % (who, list(b.shape), list(scale.shape)))
+        _one_device(who, b, scale)
+        b = _dense(b)
+        self.K, self.N = b.shape
+        self.scale = scale.contiguous()
+        L = lib()
+        self.packed = _empty(L.icx_token_weight_bytes(self.K, self.N), dtype=torch.int8, device=b.device)
+        check(L.icx_pack_token_weight(_stream(), b.data_ptr(), self.K, self.N, self.packed.data_ptr()))
+
+    @property
+    def shape(self):
+        return (self.K, self.N)
+
+
+def gpu_quantize_tokens(x):
+    """(q int8 of x's shape, scale float32 [...]) of x [..., K]: for each token the scale
+    max(max|x| / 127, 2^-126) and q = x / scale rounded to nearest even.  A token that is not finite
+    throughout has the scale NaN and zeros."""
+    who = "QuantizeTokens"
+    code = _float_code(x, who)
+    if x.dim() < 1:
+        raise IconnxError(ERR_SHAPE, "%s: x has no tokens (shape [])" % who)
+    _one_device(who, x)
+    M, K, ld, x = _rows(x)
+    q = _empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = _empty(x.shape[:-1], dtype=_F32, device=x.device)
+    check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, K, ld, q.data_ptr(), scale.data_ptr()))
+    return q, scale
+
+
+def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
+    """y [..., N] = (q @ w) * x_scale * w.scale + bias over a :class:`TokenWeight`.  x [..., K] is a float
+    tensor, quantized by token on the way (:func:`gpu_quantize_tokens`), or int8 with its
+    ``x_scale`` [...].  ``dtype``: of y (x's own; float32 for int8 x); ``bias`` float32 [N]."""
+    who = "TokenQLinear"
+    if not isinstance(w, TokenWeight):
+        raise IconnxError(ERR_INVALID, "%s: the weight must be a TokenWeight" % who)
+    if x.dtype == torch.int8:
+        code, yt = ICX_I8, dtype or _F32
+        if x_scale is None:
+            raise IconnxError(ERR_INVALID, "%s: Int8 tokens come with their scales" % who)
+        if x_scale.dtype != _F32 or x_scale.shape != x.shape[:-1]:
+            raise IconnxError(ERR_SHAPE, "%s: x_scale must be Float32 %s, got %s %s"
+                              % (who, list(x.shape[:-1]), _name(x_scale.dtype), list(x_scale.shape)))
+    else:
+        code, yt = _float_code(x, who), dtype or x.dtype
+        if x_scale is not None:
+            raise IconnxError(ERR_INVALID, "%s: x_scale goes with Int8 tokens" % who)
+    ycode = _float_code(yt, who)
+    if x.dim() < 1 or x.shape[-1] != w.K:
+        raise IconnxError(ERR_SHAPE, "%s: K mismatch — x is %s, the weight [%d,%d]" % (who, list(x.shape), w.K, w.N))
+    if bias is not None:
+        if bias.dtype != _F32 or tuple(bias.shape) != (w.N,):
+            raise IconnxError(ERR_SHAPE, "%s: bias must be Float32 [%d], got %s %s" % (who, w.N, _name(bias.dtype), list(bias.shape)))
+        bias = _dense(bias)
+    shape = x.shape[:-1] + (w.N,)
+    if out is not None and (out.dtype != yt or out.shape != shape or not out.is_contiguous()):
+        raise IconnxError(ERR_SHAPE, "%s: out must be a contiguous %s %s" % (who, _name(yt), list(shape)))
+    _one_device(who, x, x_scale, bias, out, w.packed)
+    M, K, ld, x = _rows(x)
+    if x_scale is not None:
+        x_scale = _dense(x_scale)
+    y = out if out is not None else _empty(shape, dtype=yt, device=x.device)
+    L = lib()
+    nws = L.icx_token_qlinear_workspace_size(M, K, w.N, code)
+    ws = _workspace(nws, x.device)
+    check(L.icx_token_qlinear(_stream(), x.data_ptr(), code, ld, _p(x_scale), M, K, w.N, w.packed.data_ptr(), w.scale.data_ptr(),
+                              _p(bias), y.data_ptr(), ycode, w.N, ws.data_ptr(), nws or 1))
+    return y
+
+
+class KvCache:
+    """A paged cache of keys and values in 4 or 8 bits: ``pages`` pages of ``page_size`` tokens (a
+    multiple of 16 up to 1024) of ``kv_heads`` heads of ``head_size`` values (a multiple of 32 up to 256),
+    each block of 32 values with a power-of-two scale.  It starts out as zeros.  A token's slot is
+    page * page_size + its place in the page."""
+
+    def __init__(self, pages, page_size, kv_heads, head_size, bits=4, device="cuda"):
+        self.pages, self.page_size, self.kv_heads, self.head_size, self.bits = pages, page_size, kv_heads, head_size, bits
+        self._desc = KvCacheDesc(None, pages, page_size, kv_heads, head_size, bits)
+        n = lib().icx_kv_cache_bytes(ctypes.byref(self._desc))
+        if not n:
+            raise IconnxError(ERR_UNSUPPORTED, lib().icx_last_error().decode())
+        self.data = torch.zeros(n, dtype=_U8, device=device)
+        _require_cuda(self.data)
+        self._desc.data = self.data.data_ptr()
+        self._as_parameter_ = ctypes.addressof(self._desc)  # what a pointer argument takes when given the cache
+
+
+def _slots(slots, who):
+    code = _INDEX.get(slots.dtype)
+    if code is None:
+        raise IconnxError(ERR_DTYPE, "%s: slots must be Int64 or Int32, got %s" % (who, _name(slots.dtype)))
+    if slots.dim() != 1:
+        raise IconnxError(ERR_SHAPE, "%s: slots must be 1-D (got %s)" % (who, list(slots.shape)))
+    return code, _dense(slots)
+
+
+def gpu_kv_cache_write(cache, k, v, slots):
+    """Quantizes k and v [tokens, kv_heads, head_size] (any strides with dense heads) into the cache's
+    ``slots`` [tokens]; a slot outside the cache, as -1, is passed over."""
+    who = "KvCacheWrite"
+    code = _float_code(k, who)
+    if v.dtype != k.dtype:
+        raise IconnxError(ERR_DTYPE, "%s: k is %s, v %s" % (who, _name(k.dtype), _name(v.dtype)))
+    shape = (slots.shape[0] if slots.dim() else -1, cache.kv_heads, cache.head_size)
+    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+        raise IconnxError(ERR_SHAPE, "%s: k and v must be %s (got %s and %s)" % (who, list(shape), list(k.shape), list(v.shape)))
+    sc, slots = _slots(slots, who)
+    _one_device(who, k, v, slots, cache.data)
+    k = k if k.stride(2) == 1 else k.contiguous()
+    v = v if v.stride(2) == 1 else v.contiguous()
+    check(lib().icx_kv_cache_write(_stream(), cache, k.data_ptr(), v.data_ptr(), code, shape[0], k.stride(0), k.stride(1), v.stride(0),
+                                   v.stride(1), slots.data_ptr(), sc))
+
+
+def gpu_kv_cache_read(cache, slots, dtype=torch.float32):
+    """(k, v) [tokens, kv_heads, head_size] that the cache holds at ``slots``; zeros for a slot outside it."""
+    who = "KvCacheRead"
+    code = _float_code(dtype, who)
+    sc, slots = _slots(slots, who)
+    _one_device(who, slots, cache.data)
+    shape = (slots.shape[0], cache.kv_heads, cache.head_size)
+    k = _empty(shape, dtype=dtype, device=slots.device)
+    v = _empty(shape, dtype=dtype, device=slots.device)
+    check(lib().icx_kv_cache_read(_stream(), cache, slots.data_ptr(), sc, shape[0], k.data_ptr(), v.data_ptr(), code))
+    return k, v
+
+
+_ATTENTION_PACK = struct.Struct("=QQqqqqQqQQQiiiiiiffii")
+assert _ATTENTION_PACK.size == ctypes.sizeof(KvAttention)
+
+
+def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_rows=None, scale=None, softcap=0.0, window=0,
+                           slopes=None, causal=True, out=None):
+    """Attention of q [rows, heads, head_size] over a :class:`KvCache`, of q's type.
+
+    ``page_table`` int32 [batch, width]: the pages of each sequence in order; ``lengths`` int32 [batch]:
+    its cached tokens.  Without ``q_starts`` row b belongs to sequence b (a decoding step); with it,
+    int32 [batch + 1], the rows q_starts[b] .. q_starts[b + 1] - 1 are the last tokens of sequence b, at
+    most ``max_rows`` of each (by default all).  heads is a multiple of the cached heads.  A row at position
+    p sees the tokens j <= p (``causal``) and j > p - ``window`` (0: all); scores are q.k ``scale``
+    (head_size ** -0.5), through softcap tanh(. / ``softcap``) if that is given, plus ``slopes``[head]
+    (j - p), float32.  A row that sees no token is zero; rows of ``out`` past q_starts[batch] keep what they held."""
+    who = "KvCacheAttention"
+    code = _float_code(q, who)
+    if q.dim() != 3 or q.shape[2] != cache.head_size:
+        raise IconnxError(ERR_SHAPE, "%s: q must be [rows, heads, %d] (got %s)" % (who, cache.head_size, list(q.shape)))
+    i32 = torch.int32
+    if page_table.dtype != i32 or lengths.dtype != i32 or (q_starts is not None and q_starts.dtype != i32):
+        raise IconnxError(ERR_DTYPE, "%s: page_table, lengths and q_starts must be Int32" % who)
+    batch = lengths.shape[0] if lengths.dim() == 1 else -1
+    if page_table.dim() != 2 or page_table.shape[0] != batch or (q_starts is not None and tuple(q_starts.shape) != (batch + 1,)):
+        raise IconnxError(ERR_SHAPE, "%s: page_table [batch, width], lengths [batch], q_starts [batch + 1] (got %s, %s, %s)"
+                          % (who, list(page_table.shape), list(lengths.shape), None if q_starts is None else list(q_starts.shape)))
+    rows, heads, _ = q.shape
+    if slopes is not None:
+        if slopes.dtype != _F32 or tuple(slopes.shape) != (heads,):
+            raise IconnxError(ERR_SHAPE, "%s: slopes must be Float32 [%d], got %s %s"
+                              % (who, heads, _name(slopes.dtype), list(slopes.shape)))
+        slopes = _dense(slopes)
+    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1):
+        raise IconnxError(ERR_SHAPE, "%s: out must be a %s %s with dense heads" % (who, _name(q.dtype), list(q.shape)))
+    _one_device(who, q, page_table, lengths, q_starts, slopes, out, cache.data)
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    lengths = _dense(lengths)
+    if q_starts is not None:
+        q_starts = _dense(q_starts)
+    if out is None:
+        out = _empty(q.shape, dtype=q.dtype, device=q.device)
+    if max_rows is None:
+        max_rows = 1 if q_starts is None else rows
+    args = _ATTENTION_PACK.pack(
+        q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), page_table.data_ptr(),
+        page_table.stride(0), lengths.data_ptr(), 0 if q_starts is None else q_starts.data_ptr(),
+        0 if slopes is None else slopes.data_ptr(), code, rows, batch, heads, max_rows, page_table.shape[1],
+        cache.head_size ** -0.5 if scale is None else scale, softcap, window, 1 if causal else 0)
+    L = lib()
+    nws = L.icx_kv_cache_attention_workspace_size(cache, args)
+    ws = _workspace(nws, q.device)
+    check(L.icx_kv_cache_attention(_stream(), cache, args, ws.data_ptr(), nws))
     return out
 
 

@@ -37,7 +37,16 @@ typedef enum {
 
 /* ICX_I64: Reshape shapes (graph initializers, read on the host) and Gather indices / data.
  * ICX_BOOL: one byte per element, 0 or 1 (ONNX BOOL; Equal's output, Where's condition). */
-typedef enum { ICX_I8 = 0, ICX_U8 = 1, ICX_I32 = 2, ICX_F32 = 3, ICX_I64 = 4, ICX_BOOL = 5 } icx_dtype;
+typedef enum {
+    ICX_I8 = 0,
+    ICX_U8 = 1,
+    ICX_I32 = 2,
+    ICX_F32 = 3,
+    ICX_I64 = 4,
+    ICX_BOOL = 5,
+    ICX_F16 = 6,  /* the decoder operators alone take these two */
+    ICX_BF16 = 7,
+} icx_dtype;
 
 const char* icx_status_str(int status);
 /* Message of the last failing call on this host thread ("" if none). */
@@ -320,6 +329,81 @@ int icx_attention_f32(icx_stream_t stream, const float* q, const float* k, const
                       size_t B, size_t S, size_t H, size_t D, size_t ldq, size_t ldk,
                       size_t ldv, size_t ldo, float scale, int scale_div, int scale_q,
                       float* out);
+
+/* ---- decoder operators: products by token, the quantized key / value cache ------------------
+ * No counterpart in the reference (an encoder's engine: its quantized linear has one scale a
+ * tensor, its attention no cache).  Float tensors are ICX_F32, ICX_F16 or ICX_BF16; strides are
+ * in elements and rows are dense; sums, scales and softmax statistics are f32 or int32. */
+
+/* Int8 matrix product with a scale for each token and each output channel:
+ *   s_m = max(max_k |x_mk| / 127, 2^-126), q_mk = rne(x_mk / s_m)  (the exact quotient, rounded)
+ *   y_mn = (sum_k q_mk w_kn) (s_m w_scale_n) + bias_n
+ * A token that holds an infinity or a NaN has the scale NaN and the codes 0: its outputs are NaN,
+ * the others' are not touched.  K is 1 to 131071.
+ * The weight, int8 [K, N], is packed once into icx_token_weight_bytes (16-byte aligned). */
+size_t icx_token_weight_bytes(size_t K, size_t N);
+int icx_pack_token_weight(icx_stream_t stream, const int8_t* b, size_t K, size_t N, int8_t* packed);
+/* q [M, K] dense and scale [M] of x [M, K] (row stride x_stride). */
+int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dtype, size_t M, size_t K, int64_t x_stride, int8_t* q,
+                        float* scale);
+/* x: ICX_I8 with x_scale [M] (icx_quantize_tokens' outputs, for several products over one input), or a
+ * float type with x_scale NULL, quantized on the way.  y [M, N] of y_dtype, row stride y_stride;
+ * bias [N] f32 or NULL. */
+size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N, int x_dtype);
+int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype, int64_t x_stride, const float* x_scale, size_t M,
+                      size_t K, size_t N, const int8_t* packed, const float* w_scale, const float* bias, void* y, int y_dtype,
+                      int64_t y_stride, void* workspace, size_t workspace_bytes);
+
+/* A paged cache of keys and values in 4 or 8 bits.  A head of head_size values (a multiple of 32 up to
+ * 256) is cut into blocks of 32 with a power-of-two scale 2^e each; 4 bits hold the magnitudes 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6 and a sign, 8 bits a sign, 4 bits of exponent and 3 of mantissa up to 448.  e is the
+ * least exponent for which no value of the block rounds past the largest magnitude (kept in [-125, 125]
+ * or [-117, 119]); codes round to nearest, ties to even.  A block that holds an infinity or a NaN reads
+ * back as NaN.  page_size: tokens a page, a multiple of 16 up to 1024.  data: icx_kv_cache_bytes bytes,
+ * 16-byte aligned; the layout inside is the library's own. */
+typedef struct icx_kv_cache {
+    void* data;
+    int64_t pages;
+    int32_t page_size, kv_heads, head_size, bits;
+} icx_kv_cache;
+size_t icx_kv_cache_bytes(const icx_kv_cache* cache); /* 0 for a cache that is not supported */
+/* Quantizes k, v [tokens, kv_heads, head_size] (token and head strides given) into the slots
+ * (page * page_size + place in it; ICX_I32 or ICX_I64, on the device).  A slot outside the cache, as a
+ * negative one, is passed over.  A slot named twice in one call keeps codes of either token. */
+int icx_kv_cache_write(icx_stream_t stream, const icx_kv_cache* cache, const void* k, const void* v, int dtype, size_t tokens,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       const void* slots, int slots_dtype);
+/* Reads the slots back into k, v [tokens, kv_heads, head_size] (either may be NULL); zeros for a slot
+ * outside the cache. */
+int icx_kv_cache_read(icx_stream_t stream, const icx_kv_cache* cache, const void* slots, int slots_dtype, size_t tokens, void* k,
+                      void* v, int dtype);
+
+/* Attention over the cache.  Sequence b has lengths[b] cached tokens, in the pages
+ * page_table[b * table_stride ..] in order (at most table_width of them count), and the query rows
+ * q_starts[b] .. q_starts[b + 1] - 1 of q [rows, q_heads, head_size], or row b alone where q_starts is
+ * NULL; at most max_rows rows of a sequence are done.  Query head h reads cached head
+ * h / (q_heads / kv_heads).  Row i of n stands at p = lengths[b] - n + i:
+ *   out = softmax_j(cap(scale q.k_j) + slopes[h] (j - p)) v_j  over  j <= p (causal) and j > p - window
+ * (window 0: no limit), cap(s) = softcap tanh(s / softcap) (softcap 0: none), slopes [q_heads] f32 or
+ * NULL.  A row that sees no token is zero; tokens in a page outside the cache are not seen.  Rows of
+ * out that belong to no sequence are left as they were. */
+typedef struct icx_kv_attention {
+    const void* q;
+    void* out;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    const int32_t* page_table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* q_starts;
+    const float* slopes;
+    int32_t dtype; /* of q and out */
+    int32_t rows, batch, q_heads, max_rows, table_width;
+    float scale, softcap;
+    int32_t window, causal;
+} icx_kv_attention;
+size_t icx_kv_cache_attention_workspace_size(const icx_kv_cache* cache, const icx_kv_attention* args);
+int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* cache, const icx_kv_attention* args, void* workspace,
+                           size_t workspace_bytes);
 
 /* ---- graph executor ------------------------------------------------------------------
  * Mirrors GpuGraphExecutor (src/cuda/inference/mod.rs:208-659): add_input (:306),
