@@ -140,6 +140,204 @@ __global__ void __launch_bounds__(64 * W) token_product_small_kernel(ProductArgs
     }
 }
 
+// ---- large products: 256 x 256 tiles -------------------------------------------------------------
+// Eight waves, each 128 tokens by 64 channels, K in steps of 128 bytes; both operands' steps reach
+// LDS by global_load_lds_dwordx4 (16 bytes a lane, no registers), two steps of 64 KB in LDS.  The
+// channels are the rows of the matrix instruction and the tokens its columns, so that a lane's four
+// result registers are four channels of one token; which channels a row is stands free, and row i
+// of tile t is channel 16 (i / 4) + 4 t + i % 4 of the wave's 64, which gives a lane 16 consecutive
+// ones over its four tiles: y is stored 16 bytes a lane from the registers, whole 128-byte lines
+// a wave, with no staging.
+//
+// The two waves of a SIMD (w and w + 4) run half a phase apart, one reading its fragments while the
+// other multiplies: every phase is a part of reads and one of 16 matrix instructions with a barrier after
+// each, and waves 4 to 7 wait at one barrier more before their first phase.  A step is four phases
+// (halves of the wave's tokens by halves of its channels).  The copies of step t + 1 go into the buffer
+// that step t - 1 was read from: its last reads (phase 2 of the later waves) are over one barrier before
+// the earlier waves' phase 0 of step t, where the first copies are issued; every wave waits for its own
+// copies in phase 3, one barrier before anyone reads them.  16384 x 4096 x 4096: 228 us (2.41 POP/s; the
+// 16 x 16 tiles below 3600 us).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void wait_reads() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// 16 bytes a lane from base + offset (a lane's own) to LDS at lds + 16 lane.
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// The 16-byte chunk c of a row stands at c ^ key(row) of it: the 16 rows that a fragment read takes
+// together then lie in 16 different groups of banks (two rows of 128 bytes span the banks once).
+__device__ __forceinline__ int token_key(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int channel_key(int row) { return ((row >> 1) & 1) | ((row >> 4) & 3) << 1; }
+
+// Tiles in runs of one XCD (block i runs on XCD i % 8), 8 rows of tiles deep, so that the tiles that
+// run together share their operands in its L2.
+__device__ __forceinline__ void tile_of(const ProductArgs& g, int& tm, int& tn) {
+    int i = blockIdx.x;
+    const int n = gridDim.x, each = n >> 3, more = n & 7, x = i & 7;
+    i = x * each + min(x, more) + (i >> 3);
+    const int deep = 8 * g.tiles_n;
+    const int first = i / deep * 8, rows = min(8, g.tiles_m - first);
+    tm = first + i % deep % rows;
+    tn = i % deep / rows;
+}
+
+constexpr int kBig = 256, kStep = 128;
+
+// 16 channels of one token from n on.
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int n, int N, bool wide, const float (&v)[16]) {
+    if (wide && n + 16 <= N) {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) {
+            vec w;
+#pragma unroll
+            for (int e = 0; e < 16 / (int)sizeof(T); ++e) w[e] = (T)v[i * (16 / sizeof(T)) + e];
+            *reinterpret_cast<vec*>(row + n + i * (16 / sizeof(T))) = w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (n + e < N) row[n + e] = (T)v[e];
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512, 2) token_product_big_kernel(ProductArgs g) {
+    __shared__ __attribute__((aligned(1024))) int8_t smem[2][2 * kBig * kStep];
+    int tm, tn;
+    tile_of(g, tm, tn);
+    const int m0 = tm * kBig, n0 = tn * kBig;
+    const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wid >> 2, wn = wid & 3;
+
+    // copies: 8 rows an instruction, this wave rows 32 wid .. + 31 of either operand
+    const int8_t* qa = g.q + (int64_t)m0 * g.lda;
+    const int8_t* wa = g.w + (int64_t)n0 * g.Kp;
+    uint32_t oq[4], ow[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = wid * 32 + i * 8 + (lane >> 3);
+        oq[i] = (uint32_t)((int64_t)min(row, g.M - 1 - m0) * g.lda + 16 * ((lane & 7) ^ token_key(row)));
+        ow[i] = (uint32_t)((int64_t)min(row, g.N - 1 - n0) * g.Kp + 16 * ((lane & 7) ^ channel_key(row)));
+    }
+    const uint32_t lq = lds_address(smem) + wid * 32 * kStep, lw = lq + kBig * kStep;
+    auto copy_q = [&](int buf, int kt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) copy_to_lds(qa + kt * kStep, oq[i], lq + buf * (2 * kBig * kStep) + i * 8 * kStep);
+    };
+    auto copy_w = [&](int buf, int kt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) copy_to_lds(wa + kt * kStep, ow[i], lw + buf * (2 * kBig * kStep) + i * 8 * kStep);
+    };
+    v4i acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][t] = v4i{0, 0, 0, 0};
+    v4i fq[4][2], fw[4][2];
+    auto read_q = [&](int buf, int half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = wm * 128 + half * 64 + i * 16 + lr;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                fq[i][k] = *reinterpret_cast<const v4i*>(&smem[buf][row * kStep + 16 * ((4 * k + j) ^ token_key(row))]);
+        }
+    };
+    auto read_w = [&](int buf, int half) {
+#pragma unroll
+        for (int t = 2 * half; t < 2 * half + 2; ++t) {
+            const int row = wn * 64 + (lr >> 2) * 16 + t * 4 + (lr & 3);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                fw[t][k] = *reinterpret_cast<const v4i*>(&smem[buf][kBig * kStep + row * kStep + 16 * ((4 * k + j) ^ channel_key(row))]);
+        }
+    };
+    auto multiply = [&](int hq, int hw) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 2 * hw; t < 2 * hw + 2; ++t)
+                    acc[4 * hq + i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t][k], fq[i][k], acc[4 * hq + i][t], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+    };
+
+    const int KT = g.Kp / kStep;
+    copy_q(0, 0);
+    copy_w(0, 0);
+    wait_copies();
+    barrier();
+    if (wm) barrier();
+    for (int kt = 0; kt < KT; ++kt) {
+        const int cur = kt & 1;
+        const int next = min(kt + 1, KT - 1);  // the last step again: into the buffer nobody reads any more
+        read_w(cur, 0);
+        read_q(cur, 0);
+        copy_q(cur ^ 1, next);
+        wait_reads();
+        barrier();
+        multiply(0, 0);
+        barrier();
+        read_w(cur, 1);
+        copy_w(cur ^ 1, next);
+        wait_reads();
+        barrier();
+        multiply(0, 1);
+        barrier();
+        read_q(cur, 1);
+        wait_reads();
+        barrier();
+        multiply(1, 0);
+        barrier();
+        wait_copies();
+        barrier();
+        multiply(1, 1);
+        barrier();
+    }
+    if (!wm) barrier();
+
+    const int n = n0 + wn * 64 + 16 * j;
+    float ws[16], bias[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int c = min(n + e, g.N - 1);
+        ws[e] = g.ws[c];
+        bias[e] = g.bias ? g.bias[c] : 0.0f;
+    }
+    const bool wide = (g.ldy * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int m = m0 + wm * 128 + i * 16 + lr;
+        if (m >= g.M) continue;
+        const float xs = g.xs[m];
+        float v[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[4 * t + r] = finish(acc[i][t][r], xs, ws[4 * t + r], bias[4 * t + r]);
+        store16(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, wide, v);
+    }
+}
+
 // Rows of q that are not whole steps of K (a caller's own): copied with zeros behind them.
 __global__ void __launch_bounds__(kThreads) token_pad_kernel(const int8_t* q, int64_t ld, int K, int Kp, int8_t* out) {
     const int64_t m = blockIdx.x;
@@ -261,13 +459,20 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
     g.M = (int)M;
     g.N = (int)N;
     g.Kp = (int)padded(K);
-    g.tiles_m = (int)icx::cdiv(M, 16);
-    g.tiles_n = (int)icx::cdiv(N, 16);
+    const bool big = M >= 1024 && icx::cdiv(M, kBig) * icx::cdiv(N, kBig) >= 64;
+    const size_t tile = big ? kBig : 16;
+    g.tiles_m = (int)icx::cdiv(M, tile);
+    g.tiles_n = (int)icx::cdiv(N, tile);
     if ((uint64_t)g.tiles_m * g.tiles_n * 256 > 0xffffffffull)
         ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu x %zu outputs are too many for a launch", who, M, N);
     const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n);
     return icx::with_float_type(y_dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
+        if (big) {
+            token_product_big_kernel<T><<<blocks, 512, 0, s>>>(g);
+            ICX_LAUNCH_CHECK("token_product_big_kernel");
+            return ICX_OK;
+        }
         token_product_small_kernel<4, T><<<blocks, 256, 0, s>>>(g);
         ICX_LAUNCH_CHECK("token_product_small_kernel");
         return ICX_OK;
