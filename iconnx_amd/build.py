@@ -27,8 +27,8 @@ HIP_FLAGS = [
 ]
 # host-only C++ (the graph executor) goes through hipcc for the HIP runtime headers
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall"]
-SOURCES = ["gemm.hip", "kv_attention.hip", "dql.hip", "elementwise.hip", "encoder.hip", "layout.hip", "token_linear.hip",
-           "kv_cache.hip", "executor.cpp", "memory.cpp"]
+SOURCES = ["gemm.hip", "kv_attention_f32.hip", "kv_attention_f16.hip", "kv_attention_bf16.hip", "kv_attention.hip", "dql.hip",
+           "elementwise.hip", "encoder.hip", "layout.hip", "token_linear.hip", "kv_cache.hip", "executor.cpp", "memory.cpp"]
 
 
 def _compile(src):

@@ -1,0 +1,58 @@
+// What the attention's entry point hands to its kernels, which are built in a file for each type.
+#pragma once
+
+#include "kv_format.hpp"
+
+namespace icx {
+
+struct AttnArgs {
+    const uint8_t* data;
+    icx::KvLayout l;
+    int pages, page_size;
+    const void* q;
+    int64_t q_row, q_head;  // strides, elements
+    void* out;
+    int64_t o_row, o_head;
+    const int32_t* table;
+    int64_t table_stride;
+    int width;
+    const int32_t* lengths;
+    const int32_t* starts;  // null: one row a sequence
+    int batch, group, heads_q, max_rows, rows_total;
+    float scale, softcap;
+    int window, causal;
+    const float* slopes;
+    int row_tiles, splits;
+    int big_tiles, few_rows;  // of 128 rows; sequences of at most few_rows go to the first kernel
+    float* part;   // [splits][rows_total * heads_q][D] sums of exp(s - m) v
+    float2* ml;    // [splits][rows_total * heads_q] (m, in powers of two; sum of exp)
+};
+
+// The rows and tokens of one sequence, from the device's own lengths: what is out of range is cut to it.
+struct Sequence {
+    int start, rows, len;  // rows: those that are done, at most max_rows
+    int base;              // position of the first row
+};
+__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
+    Sequence s;
+    s.start = a.starts ? a.starts[b] : b;
+    int n = 0;
+    if (s.start >= 0 && s.start <= a.rows_total) n = a.starts ? max(0, min(a.starts[b + 1], a.rows_total) - s.start) : 1;
+    s.rows = min(n, a.max_rows);
+    s.len = max(0, min(a.lengths[b], a.width * a.page_size));
+    s.base = s.len - n;
+    return s;
+}
+
+// bfloat16 numbers that a query is taken apart into, and a probability is held in.
+constexpr int attention_terms(int dtype) { return dtype == ICX_BF16 ? 1 : dtype == ICX_F16 ? 2 : 3; }
+
+// Rows of a block of kv_attention_tiles_kernel: two tiles of 16 for each wave while their queries and
+// sums fit the registers.
+constexpr int attention_tile_rows(int G, int terms) { return G * terms >= 12 ? 64 : 128; }
+
+void launch_attention_bf16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);
+void launch_attention_f16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);
+void launch_attention_f32(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);
+
+}  // namespace icx

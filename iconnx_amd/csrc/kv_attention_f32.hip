@@ -1,0 +1,6 @@
+#include "kv_attention_kernels.hpp"
+
+void icx::launch_attention_f32(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a) {
+    if (bits == 4) launch_bits<4, 3, float>(few, many, s, a);
+    else launch_bits<8, 3, float>(few, many, s, a);
+}

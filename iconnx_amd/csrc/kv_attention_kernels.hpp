@@ -1,0 +1,704 @@
+// Attention over the quantized key / value cache (kv_format.hpp has the format).
+//
+// Row i of the n rows of a sequence of L cached tokens stands at p = L - n + i.  With s_j =
+// cap(scale q.k_j) + slope (j - p) over the tokens j <= p (causal) and j > p - window,
+//   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),
+// computed in one walk over the tokens with a running maximum m and sum; a row that no token is
+// visible to is zero.  All query heads of a cached head are rows of one matrix, so a key or value is
+// read and decoded once for them.
+//
+// Both products run on v_mfma_f32_16x16x32_bf16, transposed: S^T = K Q^T leaves a lane the scores of
+// one row (column lane % 16) and of 4 tokens of a chunk of 16 (rows 4 (lane / 16) ..), and two
+// chunks give it the 8 tokens that the second product, O^T = V^T P^T, wants of it as an operand: the
+// probabilities never leave its registers.  Keys and values are exact in bfloat16.  Queries are
+// taken apart into a sum of TERMS bfloat16 numbers, exactly (1 from bfloat16, 2 from float16, 3
+// from float32), and probabilities likewise, where one term is a rounding to bfloat16's 8 bits (half
+// a step, 2^-8 of a weight, as the rounding of a bfloat16 output is; the weights' errors mostly
+// cancel), two hold 16 bits and three 24.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "internal.hpp"
+#include "kv_attention.hpp"
+#include "kv_format.hpp"
+
+namespace {
+
+using icx::AttnArgs;
+using icx::Sequence;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// v[0..7] as a sum of TERMS packed bfloat16 operands.
+template <int TERMS>
+__device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[TERMS]) {
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = v[e];
+#pragma unroll
+    for (int n = 0; n < TERMS; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const __bf16 h = (__bf16)r[e];
+            t[n][e] = h;
+            if (n + 1 < TERMS) r[e] -= (float)h;
+        }
+}
+
+// tanh to a few ulps: away from 0 through exp, near it by its series (exp's form loses digits there).
+__device__ __forceinline__ float tanh_f32(float x) {
+    const float y = fabsf(x);
+    const float z = y * y;
+    const float near = y * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
+    const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+    return copysignf(y < 0.25f ? near : far, x);
+}
+
+// The codes and scales of 32 tokens (two chunks) of one cached head, as a lane's operands need them.
+template <int BITS, int G>
+struct Tile {
+    uint32_t k[2][G * BITS / 4];
+    uint32_t v[2][G * BITS / 4];
+    uint32_t ks[2];     // the lane's keys' scales, a byte for each of its blocks
+    uint32_t vs[2][G];  // the values' scales of its 4 tokens, by block
+};
+
+// N dwords that stand at a multiple of 4 bytes, of 8 where N is even and of 16 where 4 divides it.
+template <int N>
+__device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&d)[N]) {
+    constexpr int W = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
+    typedef uint32_t vec __attribute__((ext_vector_type(W)));
+#pragma unroll
+    for (int i = 0; i < N / W; ++i) {
+        const vec w = reinterpret_cast<const vec*>(p)[i];
+#pragma unroll
+        for (int e = 0; e < W; ++e) d[W * i + e] = w[e];
+    }
+}
+
+// The lane's quarter of a key, G steps of 8 values from value 8 G j on, starts 8 (G j % 4) values into
+// block G j / 4: the scale of step i is byte (G j % 4 + i) / 4 of those loaded, and where no quarter
+// starts inside a block (or none ends past its first) that is the same byte in every lane.
+template <int G>
+constexpr bool kSameByte = G % 4 == 0 || G <= 2;
+
+template <int BITS, int G>
+__device__ __forceinline__ void load_chunk(const uint8_t* c, int lane, Tile<BITS, G>& t, int n) {
+    const int lr = lane & 15, j = lane >> 4;
+    load_dwords(c + (lr * 4 + j) * G * BITS, t.k[n]);
+    load_dwords(c + icx::kv_codes(G, BITS) + (j * 16 + lr) * G * BITS, t.v[n]);
+    load_dwords(c + icx::kv_value_scales(G, BITS) + j * 4 * G, t.vs[n]);
+    const uint8_t* sp = c + icx::kv_key_scales(G, BITS) + lr * G;
+    const int at = j * G >> 2;
+    if constexpr (G == 8) {
+        t.ks[n] = *reinterpret_cast<const uint16_t*>(sp + at);
+    } else if constexpr (kSameByte<G>) {
+        t.ks[n] = sp[at];
+    } else {
+        t.ks[n] = sp[at] | (uint32_t)sp[min(at + 1, G - 1)] << 8;
+        if constexpr (G == 7) t.ks[n] |= (uint32_t)sp[min(at + 2, G - 1)] << 16;
+    }
+}
+
+// Keys' operand of step i (values 8 (G j + i) .. + 7 of the lane's token).
+template <int BITS, int G>
+__device__ __forceinline__ bf16x8 key_operand(const Tile<BITS, G>& t, int n, int i, int j) {
+    float s;
+    if constexpr (kSameByte<G>) s = icx::scale_of(t.ks[n], i >> 2);
+    else s = icx::scale_of(t.ks[n] >> (((j * G & 3) + i) >> 2 << 3), 0);
+    u32x4 w;
+    if constexpr (BITS == 4) {
+        w[0] = icx::decode2<4, 0>(t.k[n][i], s);
+        w[1] = icx::decode2<4, 1>(t.k[n][i], s);
+        w[2] = icx::decode2<4, 2>(t.k[n][i], s);
+        w[3] = icx::decode2<4, 3>(t.k[n][i], s);
+    } else {
+        const uint32_t x = t.k[n][2 * i], y = t.k[n][2 * i + 1];
+        w[0] = icx::decode2<8, 0>(x, s);
+        w[1] = icx::decode2<8, 1>(x, s);
+        w[2] = icx::decode2<8, 0>(y, s);
+        w[3] = icx::decode2<8, 1>(y, s);
+    }
+    return __builtin_bit_cast(bf16x8, w);
+}
+
+// Values' operands of block g: rows d = 32 g + lane % 16 (lo) and 16 further (hi); the lane's 4 tokens of
+// chunk n, half of an operand's 8.
+template <int BITS, int G>
+__device__ __forceinline__ void value_halves(const Tile<BITS, G>& t, int n, int g, uint2& lo, uint2& hi) {
+    uint32_t p[4];
+    const uint32_t s = t.vs[n][g];
+    if constexpr (BITS == 4) {
+        const uint32_t w = t.v[n][g];
+        p[0] = icx::decode2<4, 0>(w, icx::scale_of(s, 0));
+        p[1] = icx::decode2<4, 1>(w, icx::scale_of(s, 1));
+        p[2] = icx::decode2<4, 2>(w, icx::scale_of(s, 2));
+        p[3] = icx::decode2<4, 3>(w, icx::scale_of(s, 3));
+    } else {
+        const uint32_t w = t.v[n][2 * g], x = t.v[n][2 * g + 1];
+        p[0] = icx::decode2<8, 0>(w, icx::scale_of(s, 0));
+        p[1] = icx::decode2<8, 1>(w, icx::scale_of(s, 1));
+        p[2] = icx::decode2<8, 0>(x, icx::scale_of(s, 2));
+        p[3] = icx::decode2<8, 1>(x, icx::scale_of(s, 3));
+    }
+    lo = make_uint2(__builtin_amdgcn_perm(p[1], p[0], 0x05040100u), __builtin_amdgcn_perm(p[3], p[2], 0x05040100u));
+    hi = make_uint2(__builtin_amdgcn_perm(p[1], p[0], 0x07060302u), __builtin_amdgcn_perm(p[3], p[2], 0x07060302u));
+}
+template <int BITS, int G>
+__device__ __forceinline__ void value_operands(const Tile<BITS, G>& t, int g, bf16x8& lo, bf16x8& hi) {
+    uint2 l0, h0, l1, h1;
+    value_halves<BITS, G>(t, 0, g, l0, h0);
+    value_halves<BITS, G>(t, 1, g, l1, h1);
+    lo = __builtin_bit_cast(bf16x8, u32x4{l0.x, l0.y, l1.x, l1.y});
+    hi = __builtin_bit_cast(bf16x8, u32x4{h0.x, h0.y, h1.x, h1.y});
+}
+
+// What a tile of 32 tokens from t0 needs beside its data.
+struct Place {
+    const uint8_t* c[2];
+    bool there[2];
+};
+__device__ __forceinline__ Place place(const AttnArgs& a, const int32_t* row, const uint8_t* head, int t0) {
+    Place p;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int chunk = (t0 >> 4) + n;
+        const int at = min(chunk / a.l.chunks, a.width - 1);
+        const int page = row[at];
+        p.there[n] = page >= 0 && page < a.pages;
+        p.c[n] = head + (int64_t)(p.there[n] ? page : 0) * a.l.page_bytes + (int64_t)(chunk % a.l.chunks) * a.l.chunk_bytes;
+    }
+    return p;
+}
+
+// One block: 16 rows (row tile rt) of one cached head of one sequence, one share of its tokens; the
+// four waves take tiles of 32 tokens in turn and are joined at the end.
+constexpr int kWaves = 4;
+
+template <int BITS, int TERMS, int G, typename T>
+__global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs a) {
+    extern __shared__ float smem[];  // [waves][16 rows][D + 4] then (m, l) [waves][16]
+    constexpr int D = 32 * G;
+    const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int x = blockIdx.x;
+    const int split = x % a.splits;
+    x /= a.splits;
+    const int rt = x % a.row_tiles;
+    x /= a.row_tiles;
+    const int h = x % a.l.heads, b = x / a.l.heads;
+    const Sequence sq = icx::sequence(a, b);
+    const int rows = sq.rows * a.group;
+    if (rows > a.few_rows || rt * 16 >= rows) return;
+    const int first = rt * 16 / a.group, last = min(rt * 16 + 15, rows - 1) / a.group;
+    const int base = sq.base;
+    const int end = a.causal ? max(0, min(sq.len, base + last + 1)) : sq.len;
+    const int begin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
+    // every row sees every token of [full_begin, full_end)
+    const int full_end = a.causal ? min(sq.len, base + first + 1) : sq.len;
+    const int full_begin = a.window > 0 ? base + last - a.window + 1 : 0;
+    const int tile0 = begin >> 5, tiles = max(0, ((end + 31) >> 5) - tile0);
+    const int share = max(kWaves, (tiles + a.splits - 1) / a.splits);
+    const int from = min(tiles, split * share), to = min(tiles, from + share);
+
+    // the lane's row
+    const int r = rt * 16 + lr;
+    const bool row_there = r < rows;
+    const int tok = min(r, rows - 1) / a.group, hq = h * a.group + min(r, rows - 1) % a.group;
+    const int p = base + tok;
+    const int lowest = a.window > 0 ? p - a.window : -1;  // a token is seen above it
+    const int highest = a.causal ? min(p, sq.len - 1) : sq.len - 1;
+    const float slope = a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    const float c = a.scale * kLog2e, cap = a.softcap * kLog2e, incap = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+
+    bf16x8 qf[G][TERMS];
+    {
+        const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(sq.start + tok) * a.q_row + (int64_t)hq * a.q_head + j * 8 * G;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (row_there) icx::load_f32(qp + 8 * i, v);
+            split_terms<TERMS>(v, qf[i]);
+        }
+    }
+
+    f32x4 acc[2 * G];
+#pragma unroll
+    for (int i = 0; i < 2 * G; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+
+    const uint8_t* head = a.data + (int64_t)h * a.l.head_bytes;
+    const int32_t* table = a.table + b * a.table_stride;
+    Tile<BITS, G> t;
+    for (int i = from + wid; i < to; i += kWaves) {
+        const int t0 = (tile0 + i) * 32;
+        const Place pl = place(a, table, head, t0);
+        load_chunk<BITS, G>(pl.c[0], lane, t, 0);
+        load_chunk<BITS, G>(pl.c[1], lane, t, 1);
+        const bool edge = t0 < full_begin || t0 + 32 > full_end || !pl.there[0] || !pl.there[1];
+
+        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const bf16x8 k = key_operand<BITS, G>(t, n, e, j);
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u) s[n] = mfma(k, qf[e][u], s[n]);
+            }
+        }
+        // scores in powers of two
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = a.softcap > 0.0f ? cap * tanh_f32(s[e >> 2][e & 3] * incap) : s[e >> 2][e & 3] * c;
+        if (a.slopes) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = fmaf(slope, (float)(t0 + 16 * (e >> 2) + 4 * j + (e & 3) - p), w[e]);
+        }
+        uint32_t spoilt = 0;  // blocks whose NaN the row sees (edge tiles)
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = t0 + 16 * (e >> 2) + 4 * j + (e & 3);
+                const bool seen = at > lowest && at <= highest && pl.there[e >> 2];
+                if (!seen) w[e] = -INFINITY;
+                // A weight of zero does not take a NaN out of the product: a NaN block counts as zeros
+                // there, and reaches the rows that see it by hand.
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t byte = 255u << (8 * (e & 3));
+                    if ((t.vs[e >> 2][g] & byte) == byte) {
+                        t.vs[e >> 2][g] &= ~byte;
+                        if (seen) spoilt |= 1u << g;
+                    }
+                }
+            }
+            spoilt |= (uint32_t)__shfl_xor((int)spoilt, 16, 64);
+            spoilt |= (uint32_t)__shfl_xor((int)spoilt, 32, 64);
+        }
+        float top = w[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, w[e]);
+        // The running maximum moves only when a score passes it by 2^8: until then the weights stay
+        // below 256 and the sums need no rescaling.
+        if (__any(top > m + 8.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float next = fmaxf(m, top);
+            const float f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < 2 * G; ++e) acc[e] *= f;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+        float pr[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            pr[e] = __builtin_amdgcn_exp2f(w[e] - mu);
+            l += pr[e];
+        }
+        bf16x8 pf[TERMS];
+        split_terms<TERMS>(pr, pf);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            bf16x8 lo, hi;
+            value_operands<BITS, G>(t, g, lo, hi);
+#pragma unroll
+            for (int u = 0; u < TERMS; ++u) {
+                acc[2 * g] = mfma(lo, pf[u], acc[2 * g]);
+                acc[2 * g + 1] = mfma(hi, pf[u], acc[2 * g + 1]);
+            }
+        }
+        if (spoilt) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (spoilt >> g & 1) {
+                    acc[2 * g] += __builtin_nanf("");
+                    acc[2 * g + 1] += __builtin_nanf("");
+                }
+        }
+    }
+
+    // join the waves
+    const int held = min(16, rows - rt * 16), stride = D + 4;
+    float2* ml = reinterpret_cast<float2*>(smem + kWaves * held * stride);
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (lane < held) ml[wid * 16 + lane] = make_float2(m, l);
+    if (lr < held) {
+        float* o = smem + (wid * held + lr) * stride + 4 * j;
+#pragma unroll
+        for (int e = 0; e < 2 * G; ++e)
+            *reinterpret_cast<f32x4*>(o + 16 * e) = acc[e];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < held * (D / 4); e += 64 * kWaves) {
+        const int row = e / (D / 4), d = e % (D / 4) * 4;
+        float top = ml[row].x;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ml[w * 16 + row].x);
+        const float mu = top == -INFINITY ? 0.0f : top;
+        f32x4 sum = {0, 0, 0, 0};
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(ml[w * 16 + row].x - mu);
+            total += f * ml[w * 16 + row].y;
+            sum += f * *reinterpret_cast<const f32x4*>(smem + (w * held + row) * stride + d);
+        }
+        const int rr = rt * 16 + row, tk = rr / a.group, qh = h * a.group + rr % a.group;
+        const int64_t at = (int64_t)(sq.start + tk) * a.heads_q + qh;
+        if (a.splits > 1) {
+            *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.rows_total * a.heads_q + at) * D + d) = sum;
+            if (d == 0) a.ml[(int64_t)split * a.rows_total * a.heads_q + at] = make_float2(top, total);
+        } else {
+            const bool any = !(total == 0.0f && top == -INFINITY);  // no token: zero
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = any ? sum[k] / total : 0.0f;
+            icx::store_f32(reinterpret_cast<T*>(a.out) + (int64_t)(sq.start + tk) * a.o_row + (int64_t)qh * a.o_head + d, v);
+        }
+    }
+}
+
+// ---- many rows ------------------------------------------------------------------------------------
+// One block: 128 rows of one cached head of one sequence (4 waves of 32; half of that where the queries'
+// terms would not leave the registers for it), one share of its tokens.
+// The waves decode a step of tokens together, a chunk of 16 each, into LDS as the bfloat16 operands of
+// both products, in the order that their lanes read them back (16 bytes a lane, in lane order, so
+// without bank conflicts); the next step's codes are on their way meanwhile, and two steps stand in LDS,
+// one barrier a step.  Decoding then costs each wave a quarter of what it does in the kernel above,
+// and an operand read from LDS serves two tiles of 16 rows.
+//
+// A NaN of a value must not meet a weight of zero in the product.  The decoder writes zeros in its
+// place and notes it; steps with such a note, which are rare, add NaN by hand to the rows that see it.
+
+template <int BITS, int TERMS, int G, typename T>
+__global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(AttnArgs a) {
+    constexpr int NQ = icx::attention_tile_rows(G, TERMS) / 64, C = 4;  // tiles of 16 rows a wave; chunks a step
+    constexpr int kTileRows = 64 * NQ;
+    constexpr int kKeys = C * G * 1024, kValues = C * G * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2][kKeys + kValues];
+    __shared__ uint32_t notes[2][C];       // of a chunk: 1 in no page of the cache, 2 holds a NaN value
+    __shared__ uint32_t spoilt[2][16 * C];  // of a token: its blocks of values that are NaN
+    const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the cached heads vary fastest (neighbouring blocks run on different XCDs, a head's own on one),
+    // then the rows from the last, which see the most tokens
+    int x = blockIdx.x;
+    const int h = x % a.l.heads;
+    x /= a.l.heads;
+    const int b = x % a.batch;
+    x /= a.batch;
+    const int split = x % a.splits;
+    const int rt = a.big_tiles - 1 - x / a.splits;
+    const Sequence sq = icx::sequence(a, b);
+    const int rows = sq.rows * a.group;
+    if (rows <= a.few_rows || rt * kTileRows >= rows) return;
+    const int base = sq.base;
+    const int r_last = min(rt * kTileRows + kTileRows - 1, rows - 1);
+    const int first = rt * kTileRows / a.group, last = r_last / a.group;
+    const int end = a.causal ? max(0, min(sq.len, base + last + 1)) : sq.len;
+    const int begin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
+    constexpr int S = 16 * C;
+    const int step0 = begin / S, steps = max(0, (end + S - 1) / S - step0);
+    const int share = (steps + a.splits - 1) / a.splits;
+    const int from = min(steps, split * share), to = min(steps, from + share);
+
+    // this wave's rows and what all of them, or any, see
+    const int w0 = rt * kTileRows + wid * 16 * NQ;
+    const bool mine = w0 < rows;
+    const int wfirst = min(w0, rows - 1) / a.group, wlast = min(w0 + 16 * NQ - 1, rows - 1) / a.group;
+    const int wend = a.causal ? min(sq.len, base + wlast + 1) : sq.len;
+    const int wbegin = a.window > 0 ? base + wfirst - a.window + 1 : 0;
+    const int full_end = a.causal ? min(sq.len, base + wfirst + 1) : sq.len;
+    const int full_begin = a.window > 0 ? base + wlast - a.window + 1 : 0;
+    int p[NQ], lowest[NQ], highest[NQ];
+    float slope[NQ];
+    // a negative scale is taken into the queries, so that the largest product has the largest score
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    const float c = fabsf(a.scale) * kLog2e, cap = a.softcap * kLog2e, incap = a.softcap > 0.0f ? fabsf(a.scale) / a.softcap : 0.0f;
+    bf16x8 qf[NQ][G][TERMS];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        const int r = min(w0 + 16 * t + lr, rows - 1), tok = r / a.group, hq = h * a.group + r % a.group;
+        p[t] = base + tok;
+        lowest[t] = a.window > 0 ? p[t] - a.window : -1;
+        highest[t] = a.causal ? min(p[t], sq.len - 1) : sq.len - 1;
+        slope[t] = a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+        const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(sq.start + tok) * a.q_row + (int64_t)hq * a.q_head + j * 8 * G;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            icx::load_f32(qp + 8 * i, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= sign;
+            split_terms<TERMS>(v, qf[t][i]);
+        }
+    }
+    f32x4 acc[NQ][2 * G];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2 * G; ++e) acc[t][e] = f32x4{0, 0, 0, 0};
+    }
+
+    const uint8_t* head = a.data + (int64_t)h * a.l.head_bytes;
+    const int32_t* table = a.table + b * a.table_stride;
+    Tile<BITS, G> raw;  // its chunk 0: this wave's chunk of the step to come
+    bool there = false;
+    auto fetch = [&](int i) {
+        const int chunk = (step0 + i) * C + wid;
+        const int at = min(chunk / a.l.chunks, a.width - 1);
+        const int page = table[at];
+        there = page >= 0 && page < a.pages;
+        const uint8_t* src = head + (int64_t)(there ? page : 0) * a.l.page_bytes + (int64_t)(chunk % a.l.chunks) * a.l.chunk_bytes;
+        load_chunk<BITS, G>(src, lane, raw, 0);
+    };
+    auto decode = [&](int buf) {
+        uint8_t* kd = smem[buf] + wid * G * 1024 + lane * 16;
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+            *reinterpret_cast<bf16x8*>(kd + e * 1024) = key_operand<BITS, G>(raw, 0, e, j);
+        }
+        uint32_t bad = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            // a byte of 255 in the scales
+            const uint32_t s = raw.vs[0][g];
+            bad |= (~s - 0x01010101u) & s & 0x80808080u;
+        }
+        const bool any = __any(bad != 0);
+        if (any) {
+            uint32_t mask[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t byte = 255u << (8 * e);
+                    if ((raw.vs[0][g] & byte) == byte) {
+                        raw.vs[0][g] &= ~byte;
+                        mask[e] |= 1u << g;
+                    }
+                }
+            }
+            if (lr == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) spoilt[buf][wid * 16 + 4 * j + e] = mask[e];
+            }
+        }
+        if (lane == 0) notes[buf][wid] = (there ? 0u : 1u) | (any ? 2u : 0u);
+        // operands of 32 tokens: this chunk's 4 tokens of a lane are one half of its 8
+        uint8_t* vd = smem[buf] + kKeys + (wid >> 1) * 2 * G * 1024 + lane * 16 + (wid & 1) * 8;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint2 lo, hi;
+            value_halves<BITS, G>(raw, 0, g, lo, hi);
+            *reinterpret_cast<uint2*>(vd + 2 * g * 1024) = lo;
+            *reinterpret_cast<uint2*>(vd + (2 * g + 1) * 1024) = hi;
+        }
+    };
+
+    if (from < to) {
+        fetch(from);
+        decode(0);
+    }
+    __syncthreads();
+    for (int i = from; i < to; ++i) {
+        const int buf = (i - from) & 1;
+        if (i + 1 < to) fetch(i + 1);
+        const int t0 = (step0 + i) * S;
+        if (mine && t0 < wend && t0 + S > wbegin) {
+            f32x4 s[NQ][C];
+            const uint8_t* ks = smem[buf] + lane * 16;
+#pragma unroll
+            for (int n = 0; n < C; ++n) {
+                if (n) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < NQ; ++t) s[t][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < G; ++e) {
+                    const bf16x8 k = *reinterpret_cast<const bf16x8*>(ks + (n * G + e) * 1024);
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                        for (int u = 0; u < TERMS; ++u) s[t][n] = mfma(k, qf[t][e][u], s[t][n]);
+                }
+            }
+            uint32_t note = 0;
+#pragma unroll
+            for (int n = 0; n < C; ++n) note |= notes[buf][n];
+            note = __builtin_amdgcn_readfirstlane(note);
+            // scores in powers of two are s times unit
+            float unit = c;
+            // (opaque, or what each element's place gives would be kept in registers over the loop)
+            int quad = 4 * j;
+            asm volatile("" : "+v"(quad));
+            if (a.softcap > 0.0f || a.slopes || c == 0.0f) {  // (a unit of 0 would make NaN of a hidden score)
+                unit = 1.0f;
+#pragma unroll
+                for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4 * C; ++e) {
+                        if ((e & 3) == 0) __builtin_amdgcn_sched_barrier(0);
+                        float w = s[t][e >> 2][e & 3];
+                        w = a.softcap > 0.0f ? cap * tanh_f32(w * incap) : w * c;
+                        s[t][e >> 2][e & 3] = fmaf(slope[t], (float)(t0 + 16 * (e >> 2) + quad + (e & 3) - p[t]), w);
+                    }
+            }
+            if (t0 < full_begin || t0 + S > full_end || note) {
+#pragma unroll
+                for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                    for (int n = 0; n < C; ++n) {
+                        const int low = lowest[t] - t0 - 16 * n, high = notes[buf][n] & 1u ? -1 : highest[t] - t0 - 16 * n;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int in = quad + e;
+                            s[t][n][e] = ((in > low) & (in <= high)) ? s[t][n][e] : -INFINITY;
+                        }
+                    }
+            }
+            float top[NQ];
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) {
+                top[t] = s[t][0][0];
+#pragma unroll
+                for (int e = 1; e < 4 * C; ++e) top[t] = fmaxf(top[t], s[t][e >> 2][e & 3]);
+                top[t] *= unit;
+            }
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) {
+                if (__any(top[t] > m[t] + 8.0f)) {
+                    top[t] = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
+                    top[t] = fmaxf(top[t], __shfl_xor(top[t], 32, 64));
+                    const float next = fmaxf(m[t], top[t]);
+                    const float f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - next);
+                    m[t] = next;
+                    l[t] *= f;
+#pragma unroll
+                    for (int e = 0; e < 2 * G; ++e) acc[t][e] *= f;
+                }
+                const float mu = m[t] == -INFINITY ? 0.0f : m[t];
+#pragma unroll
+                for (int e = 0; e < 4 * C; ++e) s[t][e >> 2][e & 3] = __builtin_amdgcn_exp2f(fmaf(s[t][e >> 2][e & 3], unit, -mu));
+#pragma unroll
+                for (int n = 0; n < C; ++n) l[t] += (s[t][n][0] + s[t][n][1]) + (s[t][n][2] + s[t][n][3]);
+            }
+            const uint8_t* vs = smem[buf] + kKeys + lane * 16;
+#pragma unroll
+            for (int n = 0; n < C / 2; ++n) {
+                __builtin_amdgcn_sched_barrier(0);
+                bf16x8 pf[NQ][TERMS];
+#pragma unroll
+                for (int t = 0; t < NQ; ++t) {
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = s[t][2 * n + (e >> 2)][e & 3];
+                    split_terms<TERMS>(w, pf[t]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2 * G; ++e) {
+                    const bf16x8 v = *reinterpret_cast<const bf16x8*>(vs + (n * 2 * G + e) * 1024);
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                        for (int u = 0; u < TERMS; ++u) acc[t][e] = mfma(v, pf[t][u], acc[t][e]);
+                }
+            }
+            if (note & 2u) {
+#pragma unroll 1
+                for (int n = 0; n < C; ++n) {
+                    if (!(notes[buf][n] & 2u) || notes[buf][n] & 1u) continue;
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t) {
+                        uint32_t nan = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int at = t0 + 16 * n + 4 * j + e;
+                            if (at > lowest[t] && at <= highest[t]) nan |= spoilt[buf][16 * n + 4 * j + e];
+                        }
+                        nan |= (uint32_t)__shfl_xor((int)nan, 16, 64);
+                        nan |= (uint32_t)__shfl_xor((int)nan, 32, 64);
+#pragma unroll
+                        for (int g = 0; g < G; ++g)
+                            if (nan >> g & 1) {
+                                acc[t][2 * g] += __builtin_nanf("");
+                                acc[t][2 * g + 1] += __builtin_nanf("");
+                            }
+                    }
+                }
+            }
+        }
+        if (i + 1 < to) decode(buf ^ 1);
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        const int r = w0 + 16 * t + lr;
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+        if (r >= rows) continue;
+        const int tok = r / a.group, hq = h * a.group + r % a.group;
+        const int64_t at = (int64_t)(sq.start + tok) * a.heads_q + hq, all = (int64_t)a.rows_total * a.heads_q;
+        if (a.splits > 1) {
+            float* o = a.part + (split * all + at) * (32 * G) + 4 * j;
+#pragma unroll
+            for (int e = 0; e < 2 * G; ++e)
+                *reinterpret_cast<f32x4*>(o + 16 * e) = acc[t][e];
+            if (j == 0) a.ml[split * all + at] = make_float2(m[t], l[t]);
+        } else {
+            const bool any = !(l[t] == 0.0f && m[t] == -INFINITY);
+            T* o = reinterpret_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.o_row + (int64_t)hq * a.o_head + 4 * j;
+            const float inv = 1.0f / l[t];
+#pragma unroll
+            for (int e = 0; e < 2 * G; ++e) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = any ? acc[t][e][k] * inv : 0.0f;
+                icx::store_f32(o + 16 * e, v);
+            }
+        }
+    }
+}
+
+// Both kernels of a call: `few` and `many` blocks of them.
+template <int BITS, int TERMS, int G, typename T>
+void launch_heads(unsigned few, unsigned many, hipStream_t s, const AttnArgs& a) {
+    const size_t held = (size_t)std::min(16, a.max_rows * a.group);
+    const size_t lds = kWaves * held * (32 * G + 4) * 4 + kWaves * 16 * 8;
+    if (few) kv_attention_rows_kernel<BITS, TERMS, G, T><<<few, 64 * kWaves, lds, s>>>(a);
+    if (many) kv_attention_tiles_kernel<BITS, TERMS, G, T><<<many, 256, 0, s>>>(a);
+}
+
+template <int BITS, int TERMS, typename T>
+void launch_bits(unsigned few, unsigned many, hipStream_t s, const AttnArgs& a) {
+    switch (a.l.G) {
+        case 1: launch_heads<BITS, TERMS, 1, T>(few, many, s, a); break;
+        case 2: launch_heads<BITS, TERMS, 2, T>(few, many, s, a); break;
+        case 3: launch_heads<BITS, TERMS, 3, T>(few, many, s, a); break;
+        case 4: launch_heads<BITS, TERMS, 4, T>(few, many, s, a); break;
+        case 5: launch_heads<BITS, TERMS, 5, T>(few, many, s, a); break;
+        case 6: launch_heads<BITS, TERMS, 6, T>(few, many, s, a); break;
+        case 7: launch_heads<BITS, TERMS, 7, T>(few, many, s, a); break;
+        default: launch_heads<BITS, TERMS, 8, T>(few, many, s, a); break;
+    }
+}
+
+}  // namespace
