@@ -14,45 +14,65 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxSplits = 64;
 
-// Joins the shares of every row: a wave a row.
-template <typename T>
+// Joins the shares of every row: a wave a row.  The lanes take a share's weight each; then 8 G lanes take
+// four values each of one share, the rest those of the next shares.
+template <int G, typename T>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(AttnArgs a) {
+    constexpr int D = 32 * G, L = G > 4 ? 64 : G > 2 ? 32 : 8 * G, N = 64 / L;  // lanes a share, shares at once
     const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int D = 32 * a.l.G;
-    const int hq = (int)(id % a.heads_q);
-    const int64_t x = id / a.heads_q;
-    const int tok = (int)(x % a.max_rows);
-    const int64_t b = x / a.max_rows;
-    if (b >= a.batch) return;
+    const int hq = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const uint32_t b = blockIdx.x / (uint32_t)a.max_rows;
+    const int tok = (int)(blockIdx.x - b * (uint32_t)a.max_rows);
     const Sequence sq = icx::sequence(a, (int)b);
-    if (tok >= sq.rows) return;
+    if (tok >= sq.rows || hq >= a.heads_q) return;
     const int64_t at = (int64_t)(sq.start + tok) * a.heads_q + hq, all = (int64_t)a.rows_total * a.heads_q;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.ml[s * all + at].x);
-    const float mu = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 e = a.ml[s * all + at];
-        total += __builtin_amdgcn_exp2f(e.x - mu) * e.y;
-    }
-    const bool any = !(total == 0.0f && top == -INFINITY);
-    for (int d = 4 * lane; d < D; d += 256) {
-        f32x4 sum = {0, 0, 0, 0};
-        for (int s = 0; s < a.splits; ++s) {
-            const float f = __builtin_amdgcn_exp2f(a.ml[s * all + at].x - mu);
-            sum += f * *reinterpret_cast<const f32x4*>(a.part + (s * all + at) * D + d);
-        }
-        float v[4];
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < a.splits) ml = a.ml[lane * all + at];
+    float top = ml.x;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = any ? sum[k] / total : 0.0f;
-        icx::store_f32(reinterpret_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.o_row + (int64_t)hq * a.o_head + d, v);
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+    float total = f * ml.y;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    const int d = lane % L * 4, first = lane / L;
+    f32x4 sum = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; s += N) {
+        const int mine = s + first;
+        const float w = __shfl(f, min(mine, 63), 64);
+        // (a share that saw no token has the weight 0, and may have left nothing to read)
+        if (mine < a.splits && d < D && w != 0.0f) sum += w * *reinterpret_cast<const f32x4*>(a.part + (mine * all + at) * D + d);
+    }
+#pragma unroll
+    for (int off = L; off < 64; off <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += __shfl_xor(sum[k], off, 64);
+    if (first || d >= D) return;
+    const bool any = !(total == 0.0f && top == -INFINITY);
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = any ? sum[k] / total : 0.0f;
+    icx::store_f32(reinterpret_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.o_row + (int64_t)hq * a.o_head + d, v);
+}
+
+template <typename T>
+void launch_join(hipStream_t s, const AttnArgs& a) {
+    const dim3 blocks((unsigned)a.batch * (unsigned)a.max_rows, (unsigned)icx::cdiv((size_t)a.heads_q, 4));
+    switch (a.l.G) {
+        case 1: kv_attention_join_kernel<1, T><<<blocks, 256, 0, s>>>(a); break;
+        case 2: kv_attention_join_kernel<2, T><<<blocks, 256, 0, s>>>(a); break;
+        case 3: kv_attention_join_kernel<3, T><<<blocks, 256, 0, s>>>(a); break;
+        case 4: kv_attention_join_kernel<4, T><<<blocks, 256, 0, s>>>(a); break;
+        case 5: kv_attention_join_kernel<5, T><<<blocks, 256, 0, s>>>(a); break;
+        case 6: kv_attention_join_kernel<6, T><<<blocks, 256, 0, s>>>(a); break;
+        case 7: kv_attention_join_kernel<7, T><<<blocks, 256, 0, s>>>(a); break;
+        default: kv_attention_join_kernel<8, T><<<blocks, 256, 0, s>>>(a); break;
     }
 }
 
 // How the call is cut: tiles of rows and shares of the tokens.
 struct Plan {
-    int row_tiles, big_tiles, few_rows, splits;
+    int row_tiles, few_rows, splits, tile_waves;
     size_t few, many, part_bytes, ml_bytes;  // blocks of either kernel, workspace
 };
 constexpr size_t kFewRows = 32;
@@ -61,17 +81,27 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     const size_t group = (size_t)(a.q_heads / c.kv_heads), most = (size_t)a.max_rows * group;
     const size_t heads = (size_t)a.batch * c.kv_heads;
     const bool many = most > kFewRows;
-    const size_t tile = (size_t)icx::attention_tile_rows(c.head_size / 32, icx::attention_terms(a.dtype));
     p.few_rows = many && a.batch == 1 ? 0 : (int)kFewRows;
     p.row_tiles = (int)icx::cdiv(std::min(most, (size_t)p.few_rows), 16);
-    p.big_tiles = many ? (int)icx::cdiv(most, tile) : 0;
-    // of all rows, no more tiles are full than this
-    const size_t full = many ? std::min(heads * p.big_tiles, icx::cdiv((size_t)a.rows * a.q_heads, tile) + heads) : heads * p.row_tiles;
+    // Tiles of all sequences together: each may end in a part of one.  Blocks of 8 waves decode a token half as
+    // often, and are taken where they still give every CU one: WIDE.
+    const int G = c.head_size / 32;
+    size_t tiles = 0;
+    p.tile_waves = 4;
+    for (int waves : {8, 4}) {
+        if (!many || (waves == 8 && G > icx::kWideHeads)) continue;
+        const size_t tile = 16 * waves * (size_t)icx::attention_wave_tiles(G, icx::attention_terms(a.dtype));
+        tiles = std::min((size_t)a.batch * icx::cdiv(most, tile), icx::cdiv((size_t)a.rows * group, tile) + a.batch);
+        p.tile_waves = waves;
+        if (c.kv_heads * icx::cdiv((size_t)a.rows * group, tile) >= (size_t)icx::num_cus()) break;
+    }
+    const size_t full = many ? c.kv_heads * tiles : heads * p.row_tiles;
     const size_t tokens = (size_t)a.table_width * c.page_size;
-    const size_t want = icx::cdiv((size_t)icx::num_cus() * (many ? 2 : 8), std::max<size_t>(full, 1));
+    const size_t want = many ? (size_t)icx::num_cus() * 8 / p.tile_waves / std::max<size_t>(full, 1)
+                             : icx::cdiv((size_t)icx::num_cus() * 8, std::max<size_t>(full, 1));
     p.splits = (int)std::max<size_t>(1, std::min({want, icx::cdiv(tokens, 256), (size_t)kMaxSplits}));
     p.few = heads * p.row_tiles * p.splits;
-    p.many = heads * p.big_tiles * p.splits;
+    p.many = c.kv_heads * tiles * p.splits;
     const size_t rows = (size_t)a.rows * a.q_heads;
     p.part_bytes = p.splits > 1 ? icx::align_up((size_t)p.splits * rows * c.head_size * 4, 256) : 0;
     p.ml_bytes = p.splits > 1 ? (size_t)p.splits * rows * 8 : 0;
@@ -149,8 +179,10 @@ extern "C" int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* c
     a.causal = args->causal;
     a.slopes = args->slopes;
     a.row_tiles = p.row_tiles;
-    a.big_tiles = p.big_tiles;
     a.few_rows = p.few_rows;
+    a.tile_waves = p.tile_waves;
+    // (exact below 2^26 chunks: the remainder of 2^32 / 64 chunks at most is then worth less than one)
+    a.chunks_inverse = a.l.chunks == 1 ? 0u : (uint32_t)((0x100000000ull + a.l.chunks - 1) / a.l.chunks);
     a.splits = p.splits;
     a.part = reinterpret_cast<float*>(ws);
     a.ml = reinterpret_cast<float2*>(reinterpret_cast<char*>(ws) + p.part_bytes);
@@ -161,9 +193,8 @@ extern "C" int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* c
     launch(cache->bits, (unsigned)p.few, (unsigned)p.many, s, a);
     ICX_LAUNCH_CHECK("kv_attention");
     if (p.splits > 1) {
-        const unsigned jb = (unsigned)icx::cdiv((size_t)args->batch * args->max_rows * args->q_heads, 4);
         icx::with_float_type(args->dtype, [&](auto* t) -> int {
-            kv_attention_join_kernel<std::remove_pointer_t<decltype(t)>><<<jb, 256, 0, s>>>(a);
+            launch_join<std::remove_pointer_t<decltype(t)>>(s, a);
             return 0;
         });
         ICX_LAUNCH_CHECK("kv_attention_join_kernel");

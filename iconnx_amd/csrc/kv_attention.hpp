@@ -23,7 +23,9 @@ struct AttnArgs {
     int window, causal;
     const float* slopes;
     int row_tiles, splits;
-    int big_tiles, few_rows;  // of 128 rows; sequences of at most few_rows go to the first kernel
+    uint32_t chunks_inverse;  // ceil(2^32 / chunks of a page), 0 for one: chunk / chunks by a multiplication
+    int tile_waves;  // of a block of kv_attention_tiles_kernel
+    int few_rows;  // sequences of at most as many (rows times group) go to kv_attention_rows_kernel
     float* part;   // [splits][rows_total * heads_q][D] sums of exp(s - m) v
     float2* ml;    // [splits][rows_total * heads_q] (m, in powers of two; sum of exp)
 };
@@ -47,9 +49,11 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
 // bfloat16 numbers that a query is taken apart into, and a probability is held in.
 constexpr int attention_terms(int dtype) { return dtype == ICX_BF16 ? 1 : dtype == ICX_F16 ? 2 : 3; }
 
-// Rows of a block of kv_attention_tiles_kernel: two tiles of 16 for each wave while their queries and
-// sums fit the registers.
-constexpr int attention_tile_rows(int G, int terms) { return G * terms >= 12 ? 64 : 128; }
+// Tiles of 16 rows of a wave of kv_attention_tiles_kernel: two while their queries and sums fit the
+// registers.
+constexpr int attention_wave_tiles(int G, int terms) { return G * terms >= 12 ? 1 : 2; }
+// Its blocks are of 4 waves, or for heads of up to 32 times this of 8 (LDS holds no more of two steps).
+constexpr int kWideHeads = 4;
 
 void launch_attention_bf16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);
 void launch_attention_f16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);

@@ -55,14 +55,16 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[TER
         }
 }
 
-// tanh to a few ulps: away from 0 through exp, near it by its series (exp's form loses digits there).
-__device__ __forceinline__ float tanh_f32(float x) {
-    const float y = fabsf(x);
-    const float z = y * y;
+// cap tanh(x), x given in units of log2(e) / 2: through exp2, and in float32 (TERMS 3) by its series near 0,
+// where that form's error, 2^-22 of the cap, is not below a score's own any more.
+template <int TERMS>
+__device__ __forceinline__ float capped(float x, float cap) {
+    const float e = __builtin_amdgcn_exp2f(x);
+    const float far = fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(e + 1.0f), cap);
+    if constexpr (TERMS < 3) return far;
+    const float y = x * (0.5f / kLog2e), z = y * y;
     const float near = y * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
-    const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-    return copysignf(y < 0.25f ? near : far, x);
+    return fabsf(y) < 0.25f ? cap * near : far;
 }
 
 // The codes and scales of 32 tokens (two chunks) of one cached head, as a lane's operands need them.
@@ -164,22 +166,18 @@ __device__ __forceinline__ void value_operands(const Tile<BITS, G>& t, int g, bf
     hi = __builtin_bit_cast(bf16x8, u32x4{h0.x, h0.y, h1.x, h1.y});
 }
 
-// What a tile of 32 tokens from t0 needs beside its data.
-struct Place {
-    const uint8_t* c[2];
-    bool there[2];
-};
-__device__ __forceinline__ Place place(const AttnArgs& a, const int32_t* row, const uint8_t* head, int t0) {
-    Place p;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int chunk = (t0 >> 4) + n;
-        const int at = min(chunk / a.l.chunks, a.width - 1);
-        const int page = row[at];
-        p.there[n] = page >= 0 && page < a.pages;
-        p.c[n] = head + (int64_t)(p.there[n] ? page : 0) * a.l.page_bytes + (int64_t)(chunk % a.l.chunks) * a.l.chunk_bytes;
-    }
-    return p;
+// The page that holds a chunk of a sequence, as its table says (the last page for chunks past the table:
+// of those no token is seen), and the chunk's place; page 0 stands in for one outside the cache.
+__device__ __forceinline__ int slot_of_chunk(const AttnArgs& a, int chunk) {
+    return a.chunks_inverse ? (int)__umulhi((uint32_t)chunk, a.chunks_inverse) : chunk;
+}
+__device__ __forceinline__ int page_of_chunk(const AttnArgs& a, const int32_t* table, int chunk) {
+    return table[min(slot_of_chunk(a, chunk), a.width - 1)];
+}
+__device__ __forceinline__ bool in_cache(const AttnArgs& a, int page) { return page >= 0 && page < a.pages; }
+__device__ __forceinline__ const uint8_t* chunk_at(const AttnArgs& a, const uint8_t* head, int page, int chunk) {
+    const int in = chunk - slot_of_chunk(a, chunk) * a.l.chunks;
+    return head + (int64_t)(in_cache(a, page) ? page : 0) * a.l.page_bytes + (int64_t)in * a.l.chunk_bytes;
 }
 
 // One block: 16 rows (row tile rt) of one cached head of one sequence, one share of its tokens; the
@@ -187,7 +185,7 @@ __device__ __forceinline__ Place place(const AttnArgs& a, const int32_t* row, co
 constexpr int kWaves = 4;
 
 template <int BITS, int TERMS, int G, typename T>
-__global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, G * TERMS <= 4 ? 3 : G * TERMS <= 12 ? 2 : 1) kv_attention_rows_kernel(AttnArgs a) {
     extern __shared__ float smem[];  // [waves][16 rows][D + 4] then (m, l) [waves][16]
     constexpr int D = 32 * G;
     const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
@@ -220,7 +218,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs
     const int lowest = a.window > 0 ? p - a.window : -1;  // a token is seen above it
     const int highest = a.causal ? min(p, sq.len - 1) : sq.len - 1;
     const float slope = a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-    const float c = a.scale * kLog2e, cap = a.softcap * kLog2e, incap = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+    const float c = a.scale * kLog2e, cap = a.softcap * kLog2e, incap = a.softcap > 0.0f ? 2.0f * kLog2e * (a.scale / a.softcap) : 0.0f;
 
     bf16x8 qf[G][TERMS];
     {
@@ -240,13 +238,24 @@ __global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs
 
     const uint8_t* head = a.data + (int64_t)h * a.l.head_bytes;
     const int32_t* table = a.table + b * a.table_stride;
-    Tile<BITS, G> t;
-    for (int i = from + wid; i < to; i += kWaves) {
+    // Two tiles' registers in turn: while one is worked on, the codes of the wave's next tile are on their
+    // way, and the page numbers of the one after it.
+    struct Next {
+        int page[2];
+    };
+    auto pages = [&](int i) {
+        const int chunk = (tile0 + min(i, to - 1)) * 2;
+        return Next{{page_of_chunk(a, table, chunk), page_of_chunk(a, table, chunk + 1)}};
+    };
+    auto fetch = [&](Tile<BITS, G>& t, int i, const Next& n) {
+        const int chunk = (tile0 + min(i, to - 1)) * 2;
+        load_chunk<BITS, G>(chunk_at(a, head, n.page[0], chunk), lane, t, 0);
+        load_chunk<BITS, G>(chunk_at(a, head, n.page[1], chunk + 1), lane, t, 1);
+    };
+    auto work = [&](Tile<BITS, G>& t, int i, const Next& pl) {
         const int t0 = (tile0 + i) * 32;
-        const Place pl = place(a, table, head, t0);
-        load_chunk<BITS, G>(pl.c[0], lane, t, 0);
-        load_chunk<BITS, G>(pl.c[1], lane, t, 1);
-        const bool edge = t0 < full_begin || t0 + 32 > full_end || !pl.there[0] || !pl.there[1];
+        const bool there[2] = {in_cache(a, pl.page[0]), in_cache(a, pl.page[1])};
+        const bool edge = t0 < full_begin || t0 + 32 > full_end || !there[0] || !there[1];
 
         f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs
         // scores in powers of two
         float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = a.softcap > 0.0f ? cap * tanh_f32(s[e >> 2][e & 3] * incap) : s[e >> 2][e & 3] * c;
+        for (int e = 0; e < 8; ++e) w[e] = a.softcap > 0.0f ? capped<TERMS>(s[e >> 2][e & 3] * incap, cap) : s[e >> 2][e & 3] * c;
         if (a.slopes) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = fmaf(slope, (float)(t0 + 16 * (e >> 2) + 4 * j + (e & 3) - p), w[e]);
@@ -271,7 +280,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int at = t0 + 16 * (e >> 2) + 4 * j + (e & 3);
-                const bool seen = at > lowest && at <= highest && pl.there[e >> 2];
+                const bool seen = at > lowest && at <= highest && there[e >> 2];
                 if (!seen) w[e] = -INFINITY;
                 // A weight of zero does not take a NaN out of the product: a NaN block counts as zeros
                 // there, and reaches the rows that see it by hand.
@@ -329,6 +338,25 @@ __global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs
                     acc[2 * g + 1] += __builtin_nanf("");
                 }
         }
+    };
+    if (from + wid < to) {
+        Tile<BITS, G> t0, t1;
+        Next n0 = pages(from + wid), n1 = pages(from + wid + kWaves);
+        fetch(t0, from + wid, n0);
+        for (int i = from + wid;;) {
+            const Next n2 = pages(i + 2 * kWaves);
+            fetch(t1, i + kWaves, n1);
+            work(t0, i, n0);
+            i += kWaves;
+            if (i >= to) break;
+            n0 = n2;
+            const Next n3 = pages(i + 2 * kWaves);
+            fetch(t0, i + kWaves, n0);
+            work(t1, i, n1);
+            i += kWaves;
+            if (i >= to) break;
+            n1 = n3;
+        }
     }
 
     // join the waves
@@ -374,45 +402,70 @@ __global__ void __launch_bounds__(64 * kWaves) kv_attention_rows_kernel(AttnArgs
 }
 
 // ---- many rows ------------------------------------------------------------------------------------
-// One block: 128 rows of one cached head of one sequence (4 waves of 32; half of that where the queries'
-// terms would not leave the registers for it), one share of its tokens.
+// One block: 32 rows a wave (16 where the queries' terms would not leave the registers for more) of one
+// cached head of one sequence, one share of its tokens.
 // The waves decode a step of tokens together, a chunk of 16 each, into LDS as the bfloat16 operands of
 // both products, in the order that their lanes read them back (16 bytes a lane, in lane order, so
 // without bank conflicts); the next step's codes are on their way meanwhile, and two steps stand in LDS,
-// one barrier a step.  Decoding then costs each wave a quarter of what it does in the kernel above,
-// and an operand read from LDS serves two tiles of 16 rows.
+// one barrier a step.  An operand read from LDS serves two tiles of 16 rows, and decoding costs each wave a
+// quarter of what it does in the kernel above, or, in blocks of 8 waves, an eighth.  The sums of the
+// weights are a product with ones, of the weights as they are multiplied with the values.
+//
+// What bounds it is vector instructions: a step of 64 tokens is 64 matrix instructions of 16 cycles a wave
+// for heads of 128 from bfloat16, and 270 vector ones and 32 exponentials (of four cycles and
+// sixteen), a third of them decoding, before the 8 waves and the product with ones.
 //
 // A NaN of a value must not meet a weight of zero in the product.  The decoder writes zeros in its
 // place and notes it; steps with such a note, which are rare, add NaN by hand to the rows that see it.
 
-template <int BITS, int TERMS, int G, typename T>
-__global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(AttnArgs a) {
-    constexpr int NQ = icx::attention_tile_rows(G, TERMS) / 64, C = 4;  // tiles of 16 rows a wave; chunks a step
-    constexpr int kTileRows = 64 * NQ;
-    constexpr int kKeys = C * G * 1024, kValues = C * G * 1024;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2][kKeys + kValues];
-    __shared__ uint32_t notes[2][C];       // of a chunk: 1 in no page of the cache, 2 holds a NaN value
-    __shared__ uint32_t spoilt[2][16 * C];  // of a token: its blocks of values that are NaN
+template <int BITS, int TERMS, int G, int W, typename T>
+__global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kernel(AttnArgs a) {
+    constexpr int NQ = icx::attention_wave_tiles(G, TERMS), C = 4;  // tiles of 16 rows a wave; chunks worked on at once
+    constexpr int kTileRows = 16 * NQ * W;
+    constexpr int kKeys = C * G * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2][W / C][2 * kKeys];  // of 64 tokens keys', then values'
+    __shared__ uint32_t notes[2][W];        // of a chunk: 1 in no page of the cache, 2 holds a NaN value
+    __shared__ uint32_t spoilt[2][16 * W];  // of a token: its blocks of values that are NaN
     const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // the cached heads vary fastest (neighbouring blocks run on different XCDs, a head's own on one),
-    // then the rows from the last, which see the most tokens
+    // The cached heads vary fastest (neighbouring blocks run on different XCDs, and with 8 heads a head's own
+    // on one), then the shares, then the tiles of all sequences in one list, those of a sequence from its last
+    // rows, which see the most tokens.  (Tiles by their place in the longest sequence instead, absent ones
+    // leaving at once, load the XCDs unevenly: ragged chunks of up to 300 rows 53 us, with the list
+    // LISTED us.)
     int x = blockIdx.x;
     const int h = x % a.l.heads;
     x /= a.l.heads;
-    const int b = x % a.batch;
-    x /= a.batch;
     const int split = x % a.splits;
-    const int rt = a.big_tiles - 1 - x / a.splits;
+    x /= a.splits;
+    int b = -1, rt = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int n = b0 + lane < a.batch ? icx::sequence(a, b0 + lane).rows * a.group : 0;
+        const int own = n > a.few_rows ? (n + kTileRows - 1) / kTileRows : 0;
+        int sum = own;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int up = __shfl_up(sum, off, 64);
+            if (lane >= off) sum += up;
+        }
+        const uint64_t past = __ballot(sum > x);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            b = b0 + at;
+            rt = __builtin_amdgcn_readlane(sum, at) - 1 - x;
+            break;
+        }
+        x -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    if (b < 0) return;
     const Sequence sq = icx::sequence(a, b);
     const int rows = sq.rows * a.group;
-    if (rows <= a.few_rows || rt * kTileRows >= rows) return;
     const int base = sq.base;
     const int r_last = min(rt * kTileRows + kTileRows - 1, rows - 1);
     const int first = rt * kTileRows / a.group, last = r_last / a.group;
     const int end = a.causal ? max(0, min(sq.len, base + last + 1)) : sq.len;
     const int begin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
-    constexpr int S = 16 * C;
+    constexpr int S = 16 * W;
     const int step0 = begin / S, steps = max(0, (end + S - 1) / S - step0);
     const int share = (steps + a.splits - 1) / a.splits;
     const int from = min(steps, split * share), to = min(steps, from + share);
@@ -429,8 +482,9 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
     float slope[NQ];
     // a negative scale is taken into the queries, so that the largest product has the largest score
     const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
-    const float c = fabsf(a.scale) * kLog2e, cap = a.softcap * kLog2e, incap = a.softcap > 0.0f ? fabsf(a.scale) / a.softcap : 0.0f;
-    bf16x8 qf[NQ][G][TERMS];
+    const float c = fabsf(a.scale) * kLog2e, cap = a.softcap * kLog2e, incap = a.softcap > 0.0f ? 2.0f * kLog2e * (fabsf(a.scale) / a.softcap) : 0.0f;
+    const bool curved = a.softcap > 0.0f || a.slopes || c == 0.0f;  // (a unit of 0 would make NaN of a hidden score)
+    const T* qp[NQ];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
         const int r = min(w0 + 16 * t + lr, rows - 1), tok = r / a.group, hq = h * a.group + r % a.group;
@@ -438,22 +492,16 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
         lowest[t] = a.window > 0 ? p[t] - a.window : -1;
         highest[t] = a.causal ? min(p[t], sq.len - 1) : sq.len - 1;
         slope[t] = a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-        const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(sq.start + tok) * a.q_row + (int64_t)hq * a.q_head + j * 8 * G;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            icx::load_f32(qp + 8 * i, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= sign;
-            split_terms<TERMS>(v, qf[t][i]);
-        }
+        qp[t] = reinterpret_cast<const T*>(a.q) + (int64_t)(sq.start + tok) * a.q_row + (int64_t)hq * a.q_head + j * 8 * G;
     }
     f32x4 acc[NQ][2 * G];
-    float m[NQ], l[NQ];
+    f32x4 l[NQ];  // sums of the weights, the same in all four
+    float m[NQ];
+    const bf16x8 ones = {(__bf16)1.0f, (__bf16)1.0f, (__bf16)1.0f, (__bf16)1.0f, (__bf16)1.0f, (__bf16)1.0f, (__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
         m[t] = -INFINITY;
-        l[t] = 0.0f;
+        l[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 2 * G; ++e) acc[t][e] = f32x4{0, 0, 0, 0};
     }
@@ -462,16 +510,21 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
     const int32_t* table = a.table + b * a.table_stride;
     Tile<BITS, G> raw;  // its chunk 0: this wave's chunk of the step to come
     bool there = false;
-    auto fetch = [&](int i) {
-        const int chunk = (step0 + i) * C + wid;
-        const int at = min(chunk / a.l.chunks, a.width - 1);
-        const int page = table[at];
-        there = page >= 0 && page < a.pages;
-        const uint8_t* src = head + (int64_t)(there ? page : 0) * a.l.page_bytes + (int64_t)(chunk % a.l.chunks) * a.l.chunk_bytes;
-        load_chunk<BITS, G>(src, lane, raw, 0);
+    // (through a vector register: a scalar load on its way would keep the reads of LDS, which count with it
+    // but come in order, from being waited for one by one)
+    auto page = [&](int i) {
+        int chunk = (step0 + min(i, to - 1)) * W + wid;
+        asm volatile("" : "+v"(chunk));
+        return page_of_chunk(a, table, chunk);
+    };
+    auto fetch = [&](int i, int page) {
+        const int chunk = (step0 + i) * W + wid;
+        page = __builtin_amdgcn_readfirstlane(page);
+        there = in_cache(a, page);
+        load_chunk<BITS, G>(chunk_at(a, head, page, chunk), lane, raw, 0);
     };
     auto decode = [&](int buf) {
-        uint8_t* kd = smem[buf] + wid * G * 1024 + lane * 16;
+        uint8_t* kd = smem[buf][wid / C] + (wid % C) * G * 1024 + lane * 16;
 #pragma unroll
         for (int e = 0; e < G; ++e) {
             *reinterpret_cast<bf16x8*>(kd + e * 1024) = key_operand<BITS, G>(raw, 0, e, j);
@@ -504,7 +557,7 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
         }
         if (lane == 0) notes[buf][wid] = (there ? 0u : 1u) | (any ? 2u : 0u);
         // operands of 32 tokens: this chunk's 4 tokens of a lane are one half of its 8
-        uint8_t* vd = smem[buf] + kKeys + (wid >> 1) * 2 * G * 1024 + lane * 16 + (wid & 1) * 8;
+        uint8_t* vd = smem[buf][wid / C] + kKeys + (wid % C >> 1) * 2 * G * 1024 + lane * 16 + (wid & 1) * 8;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             uint2 lo, hi;
@@ -514,59 +567,103 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
         }
     };
 
+    // the first codes are asked for before the queries, which are used before them
+    int next = 0;
     if (from < to) {
-        fetch(from);
-        decode(0);
+        const int page0 = page(from);
+        next = page(from + 1);
+        fetch(from, page0);
     }
+    bf16x8 qf[NQ][G][TERMS];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float v[8];
+            icx::load_f32(qp[t] + 8 * i, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= sign;
+            split_terms<TERMS>(v, qf[t][i]);
+        }
+    if (from < to) decode(0);
     __syncthreads();
     for (int i = from; i < to; ++i) {
         const int buf = (i - from) & 1;
-        if (i + 1 < to) fetch(i + 1);
-        const int t0 = (step0 + i) * S;
-        if (mine && t0 < wend && t0 + S > wbegin) {
+        if (i + 1 < to) {
+            fetch(i + 1, next);
+            next = page(i + 2);
+        }
+#pragma unroll 1
+        for (int part = 0; part < W / C; ++part) {
+            const int t0 = (step0 + i) * S + part * 16 * C;
+            if (!mine || t0 >= wend || t0 + 16 * C <= wbegin) continue;
+            // Operands are read a group ahead of the products that take them: the keys of a chunk, or half of
+            // the values of 32 tokens.
+            bf16x8 f[2][G];
+            const uint8_t* operands = smem[buf][part] + lane * 16;
+            auto read = [&](int group) {
+#pragma unroll
+                for (int e = 0; e < G; ++e) f[group & 1][e] = *reinterpret_cast<const bf16x8*>(operands + (group * G + e) * 1024);
+            };
             f32x4 s[NQ][C];
-            const uint8_t* ks = smem[buf] + lane * 16;
+            read(0);
 #pragma unroll
             for (int n = 0; n < C; ++n) {
-                if (n) __builtin_amdgcn_sched_barrier(0);
+                read(n + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < NQ; ++t) s[t][n] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < G; ++e) {
-                    const bf16x8 k = *reinterpret_cast<const bf16x8*>(ks + (n * G + e) * 1024);
+                for (int e = 0; e < G; ++e)
 #pragma unroll
                     for (int t = 0; t < NQ; ++t)
 #pragma unroll
-                        for (int u = 0; u < TERMS; ++u) s[t][n] = mfma(k, qf[t][e][u], s[t][n]);
-                }
+                        for (int u = 0; u < TERMS; ++u) s[t][n] = mfma(f[n & 1][e], qf[t][e][u], s[t][n]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             uint32_t note = 0;
 #pragma unroll
-            for (int n = 0; n < C; ++n) note |= notes[buf][n];
+            for (int n = 0; n < C; ++n) note |= notes[buf][part * C + n];
             note = __builtin_amdgcn_readfirstlane(note);
             // scores in powers of two are s times unit
             float unit = c;
             // (opaque, or what each element's place gives would be kept in registers over the loop)
             int quad = 4 * j;
             asm volatile("" : "+v"(quad));
-            if (a.softcap > 0.0f || a.slopes || c == 0.0f) {  // (a unit of 0 would make NaN of a hidden score)
+            if (curved) {
                 unit = 1.0f;
+                if (a.softcap > 0.0f) {
 #pragma unroll
-                for (int t = 0; t < NQ; ++t)
+                    for (int t = 0; t < NQ; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4 * C; ++e) {
-                        if ((e & 3) == 0) __builtin_amdgcn_sched_barrier(0);
-                        float w = s[t][e >> 2][e & 3];
-                        w = a.softcap > 0.0f ? cap * tanh_f32(w * incap) : w * c;
-                        s[t][e >> 2][e & 3] = fmaf(slope[t], (float)(t0 + 16 * (e >> 2) + quad + (e & 3) - p[t]), w);
-                    }
+                        for (int n = 0; n < C; ++n) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[t][n][e] = capped<TERMS>(s[t][n][e] * incap, cap);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                        for (int n = 0; n < C; ++n) s[t][n] *= c;
+                }
+                if (a.slopes) {
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                        for (int n = 0; n < C; ++n) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[t][n][e] = fmaf(slope[t], (float)(t0 + 16 * n + quad + e - p[t]), s[t][n][e]);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                }
             }
-            if (t0 < full_begin || t0 + S > full_end || note) {
+            if (t0 < full_begin || t0 + 16 * C > full_end || note) {
 #pragma unroll
                 for (int t = 0; t < NQ; ++t)
 #pragma unroll
                     for (int n = 0; n < C; ++n) {
-                        const int low = lowest[t] - t0 - 16 * n, high = notes[buf][n] & 1u ? -1 : highest[t] - t0 - 16 * n;
+                        const int low = lowest[t] - t0 - 16 * n, high = notes[buf][part * C + n] & 1u ? -1 : highest[t] - t0 - 16 * n;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int in = quad + e;
@@ -597,13 +694,9 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
                 const float mu = m[t] == -INFINITY ? 0.0f : m[t];
 #pragma unroll
                 for (int e = 0; e < 4 * C; ++e) s[t][e >> 2][e & 3] = __builtin_amdgcn_exp2f(fmaf(s[t][e >> 2][e & 3], unit, -mu));
-#pragma unroll
-                for (int n = 0; n < C; ++n) l[t] += (s[t][n][0] + s[t][n][1]) + (s[t][n][2] + s[t][n][3]);
             }
-            const uint8_t* vs = smem[buf] + kKeys + lane * 16;
 #pragma unroll
             for (int n = 0; n < C / 2; ++n) {
-                __builtin_amdgcn_sched_barrier(0);
                 bf16x8 pf[NQ][TERMS];
 #pragma unroll
                 for (int t = 0; t < NQ; ++t) {
@@ -611,27 +704,35 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[e] = s[t][2 * n + (e >> 2)][e & 3];
                     split_terms<TERMS>(w, pf[t]);
+#pragma unroll
+                    for (int u = 0; u < TERMS; ++u) l[t] = mfma(ones, pf[t][u], l[t]);
                 }
 #pragma unroll
-                for (int e = 0; e < 2 * G; ++e) {
-                    const bf16x8 v = *reinterpret_cast<const bf16x8*>(vs + (n * 2 * G + e) * 1024);
+                for (int half = 0; half < 2; ++half) {
+                    const int group = C + 2 * n + half;
+                    if (group + 1 < 2 * C) read(group + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int t = 0; t < NQ; ++t)
+                    for (int e = 0; e < G; ++e)
 #pragma unroll
-                        for (int u = 0; u < TERMS; ++u) acc[t][e] = mfma(v, pf[t][u], acc[t][e]);
+                        for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                            for (int u = 0; u < TERMS; ++u) acc[t][half * G + e] = mfma(f[group & 1][e], pf[t][u], acc[t][half * G + e]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (note & 2u) {
 #pragma unroll 1
                 for (int n = 0; n < C; ++n) {
-                    if (!(notes[buf][n] & 2u) || notes[buf][n] & 1u) continue;
+                    const uint32_t chunk = notes[buf][part * C + n];
+                    if (!(chunk & 2u) || chunk & 1u) continue;
 #pragma unroll
                     for (int t = 0; t < NQ; ++t) {
                         uint32_t nan = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int at = t0 + 16 * n + 4 * j + e;
-                            if (at > lowest[t] && at <= highest[t]) nan |= spoilt[buf][16 * n + 4 * j + e];
+                            if (at > lowest[t] && at <= highest[t]) nan |= spoilt[buf][16 * (part * C + n) + 4 * j + e];
                         }
                         nan |= (uint32_t)__shfl_xor((int)nan, 16, 64);
                         nan |= (uint32_t)__shfl_xor((int)nan, 32, 64);
@@ -652,8 +753,6 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
         const int r = w0 + 16 * t + lr;
-        l[t] += __shfl_xor(l[t], 16, 64);
-        l[t] += __shfl_xor(l[t], 32, 64);
         if (r >= rows) continue;
         const int tok = r / a.group, hq = h * a.group + r % a.group;
         const int64_t at = (int64_t)(sq.start + tok) * a.heads_q + hq, all = (int64_t)a.rows_total * a.heads_q;
@@ -662,11 +761,11 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
 #pragma unroll
             for (int e = 0; e < 2 * G; ++e)
                 *reinterpret_cast<f32x4*>(o + 16 * e) = acc[t][e];
-            if (j == 0) a.ml[split * all + at] = make_float2(m[t], l[t]);
+            if (j == 0) a.ml[split * all + at] = make_float2(m[t], l[t][0]);
         } else {
-            const bool any = !(l[t] == 0.0f && m[t] == -INFINITY);
+            const bool any = !(l[t][0] == 0.0f && m[t] == -INFINITY);
             T* o = reinterpret_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.o_row + (int64_t)hq * a.o_head + 4 * j;
-            const float inv = 1.0f / l[t];
+            const float inv = 1.0f / l[t][0];
 #pragma unroll
             for (int e = 0; e < 2 * G; ++e) {
                 float v[4];
@@ -678,13 +777,22 @@ __global__ void __launch_bounds__(256, G > 4 ? 1 : 2) kv_attention_tiles_kernel(
     }
 }
 
-// Both kernels of a call: `few` and `many` blocks of them.
+// Both kernels of a call: `few` and `many` blocks of them.  (One kernel of both bodies would save a launch,
+// 4 us, but has too few scalar registers for them: 4096 rows over 8192 tokens 451 -> 532 us.)
 template <int BITS, int TERMS, int G, typename T>
 void launch_heads(unsigned few, unsigned many, hipStream_t s, const AttnArgs& a) {
-    const size_t held = (size_t)std::min(16, a.max_rows * a.group);
-    const size_t lds = kWaves * held * (32 * G + 4) * 4 + kWaves * 16 * 8;
-    if (few) kv_attention_rows_kernel<BITS, TERMS, G, T><<<few, 64 * kWaves, lds, s>>>(a);
-    if (many) kv_attention_tiles_kernel<BITS, TERMS, G, T><<<many, 256, 0, s>>>(a);
+    if (few) {
+        const size_t held = (size_t)std::min(16, a.max_rows * a.group);
+        const size_t lds = kWaves * held * (32 * G + 4) * 4 + kWaves * 16 * 8;
+        kv_attention_rows_kernel<BITS, TERMS, G, T><<<few, 64 * kWaves, lds, s>>>(a);
+    }
+    if constexpr (G <= icx::kWideHeads) {
+        if (many && a.tile_waves == 8) {
+            kv_attention_tiles_kernel<BITS, TERMS, G, 8, T><<<many, 512, 0, s>>>(a);
+            return;
+        }
+    }
+    if (many) kv_attention_tiles_kernel<BITS, TERMS, G, 4, T><<<many, 256, 0, s>>>(a);
 }
 
 template <int BITS, int TERMS, typename T>
