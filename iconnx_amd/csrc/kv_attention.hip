@@ -14,27 +14,41 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxSplits = 64;
 
-// Joins the shares of every row: a wave a row.  The lanes take a share's weight each; then 8 G lanes take
-// four values each of one share, the rest those of the next shares.
+// Joins the shares of every row: a block for each token of q that belongs to a sequence and 8 heads, a wave a
+// head.  The lanes take a share's weight each; then 8 G lanes take four values each of one share, the
+// rest those of the next shares.
+constexpr int kJoinWaves = 8;
+
 template <int G, typename T>
-__global__ void __launch_bounds__(256) kv_attention_join_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * kJoinWaves) kv_attention_join_kernel(AttnArgs a) {
     constexpr int D = 32 * G, L = G > 4 ? 64 : G > 2 ? 32 : 8 * G, N = 64 / L;  // lanes a share, shares at once
     const int lane = threadIdx.x & 63;
-    const int hq = blockIdx.y * 4 + (threadIdx.x >> 6);
-    const uint32_t b = blockIdx.x / (uint32_t)a.max_rows;
-    const int tok = (int)(blockIdx.x - b * (uint32_t)a.max_rows);
-    const Sequence sq = icx::sequence(a, (int)b);
-    if (tok >= sq.rows || hq >= a.heads_q) return;
-    const int64_t at = (int64_t)(sq.start + tok) * a.heads_q + hq, all = (int64_t)a.rows_total * a.heads_q;
+    const int token = blockIdx.x;
+    bool own = false;
+    for (int b0 = a.starts ? 0 : token; b0 < a.batch; b0 += 64) {
+        bool mine = false;
+        if (b0 + lane < a.batch) {
+            const Sequence sq = icx::sequence(a, b0 + lane);
+            mine = token >= sq.start && token < sq.start + sq.rows;
+        }
+        own = __any(mine);
+        if (own || !a.starts) break;
+    }
+    const int hq = blockIdx.y * kJoinWaves + (threadIdx.x >> 6);
+    if (!own || hq >= a.heads_q) return;
+    const int64_t all = (int64_t)a.rows_total * a.heads_q;
+    const int64_t at = (int64_t)token * a.heads_q + hq;
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (lane < a.splits) ml = a.ml[lane * all + at];
+    // over as many lanes as there are shares: each exchange costs as much as a load from L2 takes to start
+    const int half = a.splits > 1 ? 1 << (31 - __builtin_clz(a.splits - 1)) : 0;
     float top = ml.x;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    for (int off = half; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    top = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
     const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
     float total = f * ml.y;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    for (int off = half; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    total = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(total)));
     const int d = lane % L * 4, first = lane / L;
     f32x4 sum = {0, 0, 0, 0};
     for (int s = 0; s < a.splits; s += N) {
@@ -52,21 +66,22 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(AttnArgs a) {
     float v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = any ? sum[k] / total : 0.0f;
-    icx::store_f32(reinterpret_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.o_row + (int64_t)hq * a.o_head + d, v);
+    icx::store_f32(reinterpret_cast<T*>(a.out) + (int64_t)token * a.o_row + (int64_t)hq * a.o_head + d, v);
 }
 
 template <typename T>
 void launch_join(hipStream_t s, const AttnArgs& a) {
-    const dim3 blocks((unsigned)a.batch * (unsigned)a.max_rows, (unsigned)icx::cdiv((size_t)a.heads_q, 4));
+    const dim3 blocks((unsigned)a.rows_total, (unsigned)icx::cdiv((size_t)a.heads_q, kJoinWaves));
+    const unsigned threads = 64 * (unsigned)std::min(kJoinWaves, a.heads_q);
     switch (a.l.G) {
-        case 1: kv_attention_join_kernel<1, T><<<blocks, 256, 0, s>>>(a); break;
-        case 2: kv_attention_join_kernel<2, T><<<blocks, 256, 0, s>>>(a); break;
-        case 3: kv_attention_join_kernel<3, T><<<blocks, 256, 0, s>>>(a); break;
-        case 4: kv_attention_join_kernel<4, T><<<blocks, 256, 0, s>>>(a); break;
-        case 5: kv_attention_join_kernel<5, T><<<blocks, 256, 0, s>>>(a); break;
-        case 6: kv_attention_join_kernel<6, T><<<blocks, 256, 0, s>>>(a); break;
-        case 7: kv_attention_join_kernel<7, T><<<blocks, 256, 0, s>>>(a); break;
-        default: kv_attention_join_kernel<8, T><<<blocks, 256, 0, s>>>(a); break;
+        case 1: kv_attention_join_kernel<1, T><<<blocks, threads, 0, s>>>(a); break;
+        case 2: kv_attention_join_kernel<2, T><<<blocks, threads, 0, s>>>(a); break;
+        case 3: kv_attention_join_kernel<3, T><<<blocks, threads, 0, s>>>(a); break;
+        case 4: kv_attention_join_kernel<4, T><<<blocks, threads, 0, s>>>(a); break;
+        case 5: kv_attention_join_kernel<5, T><<<blocks, threads, 0, s>>>(a); break;
+        case 6: kv_attention_join_kernel<6, T><<<blocks, threads, 0, s>>>(a); break;
+        case 7: kv_attention_join_kernel<7, T><<<blocks, threads, 0, s>>>(a); break;
+        default: kv_attention_join_kernel<8, T><<<blocks, threads, 0, s>>>(a); break;
     }
 }
 
@@ -81,7 +96,9 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     const size_t group = (size_t)(a.q_heads / c.kv_heads), most = (size_t)a.max_rows * group;
     const size_t heads = (size_t)a.batch * c.kv_heads;
     const bool many = most > kFewRows;
-    p.few_rows = many && a.batch == 1 ? 0 : (int)kFewRows;
+    // Beside sequences of many rows, those of few have a kernel of their own where they may well be most of
+    // the batch; else, and in a batch of one, the launch (4 us) costs more than it gives.
+    p.few_rows = many && (a.batch == 1 || (size_t)a.rows * group > 2 * kFewRows * a.batch) ? 0 : (int)kFewRows;
     p.row_tiles = (int)icx::cdiv(std::min(most, (size_t)p.few_rows), 16);
     // Tiles of all sequences together: each may end in a part of one.  Blocks of 8 waves decode a token half as
     // often, and are taken where they still give every CU one: WIDE.
@@ -148,7 +165,7 @@ extern "C" int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* c
     if (!args->q || !args->out || !args->lengths || (!args->page_table && args->table_width))
         ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null q, out, page_table or lengths", who);
     const Plan p = plan_of(*cache, *args);
-    if ((p.few | p.many) > 0xffffffull || (uint64_t)args->batch * args->max_rows * args->q_heads * 64 > 0xffffffffull)
+    if ((p.few | p.many) > 0xffffffull || (uint64_t)args->rows * 64 * kJoinWaves > 0xffffffffull)
         ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %d sequences of up to %d rows are too many for a launch", who, args->batch, args->max_rows);
     if (p.part_bytes && (!ws || ws_bytes < p.part_bytes + p.ml_bytes))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, p.part_bytes + p.ml_bytes, ws_bytes);

@@ -184,8 +184,15 @@ __device__ __forceinline__ const uint8_t* chunk_at(const AttnArgs& a, const uint
 // four waves take tiles of 32 tokens in turn and are joined at the end.
 constexpr int kWaves = 4;
 
+// Waves a SIMD that its registers are kept to: sums, queries, two tiles of codes, and about 55 more.  (64
+// sequences of up to 8192 tokens, 4 bits, heads of 128: 104 us with the two that the compiler takes, 88 with three.)
+constexpr int rows_kernel_waves(int bits, int terms, int G) {
+    const int registers = 8 * G + 4 * G * terms + 4 * (G * bits / 2 + G + 1) + 55;
+    return registers <= 160 ? 3 : registers <= 225 ? 2 : 1;
+}
+
 template <int BITS, int TERMS, int G, typename T>
-__global__ void __launch_bounds__(64 * kWaves, G * TERMS <= 4 ? 3 : G * TERMS <= 12 ? 2 : 1) kv_attention_rows_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, rows_kernel_waves(BITS, TERMS, G)) kv_attention_rows_kernel(AttnArgs a) {
     extern __shared__ float smem[];  // [waves][16 rows][D + 4] then (m, l) [waves][16]
     constexpr int D = 32 * G;
     const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
@@ -423,6 +430,7 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
     constexpr int NQ = icx::attention_wave_tiles(G, TERMS), C = 4;  // tiles of 16 rows a wave; chunks worked on at once
     constexpr int kTileRows = 16 * NQ * W;
     constexpr int kKeys = C * G * 1024;
+    constexpr bool kAhead = NQ == 1 || (G <= 4 ? G * (TERMS + 2) <= 12 : G <= 6);  // (else it would not fit them)
     __shared__ __attribute__((aligned(16))) uint8_t smem[2][W / C][2 * kKeys];  // of 64 tokens keys', then values'
     __shared__ uint32_t notes[2][W];        // of a chunk: 1 in no page of the cache, 2 holds a NaN value
     __shared__ uint32_t spoilt[2][16 * W];  // of a token: its blocks of values that are NaN
@@ -432,15 +440,18 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
     // on one), then the shares, then the tiles of all sequences in one list, those of a sequence from its last
     // rows, which see the most tokens.  (Tiles by their place in the longest sequence instead, absent ones
     // leaving at once, load the XCDs unevenly: ragged chunks of up to 300 rows 53 us, with the list
-    // LISTED us.)
+    // 38 us.)
     int x = blockIdx.x;
     const int h = x % a.l.heads;
     x /= a.l.heads;
     const int split = x % a.splits;
     x /= a.splits;
     int b = -1, rt = 0;
+    Sequence sq{};
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int n = b0 + lane < a.batch ? icx::sequence(a, b0 + lane).rows * a.group : 0;
+        Sequence one{};
+        if (b0 + lane < a.batch) one = icx::sequence(a, b0 + lane);
+        const int n = one.rows * a.group;
         const int own = n > a.few_rows ? (n + kTileRows - 1) / kTileRows : 0;
         int sum = own;
 #pragma unroll
@@ -453,12 +464,15 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
             const int at = __builtin_ctzll(past);
             b = b0 + at;
             rt = __builtin_amdgcn_readlane(sum, at) - 1 - x;
+            sq.start = __builtin_amdgcn_readlane(one.start, at);
+            sq.rows = __builtin_amdgcn_readlane(one.rows, at);
+            sq.len = __builtin_amdgcn_readlane(one.len, at);
+            sq.base = __builtin_amdgcn_readlane(one.base, at);
             break;
         }
         x -= __builtin_amdgcn_readlane(sum, 63);
     }
     if (b < 0) return;
-    const Sequence sq = icx::sequence(a, b);
     const int rows = sq.rows * a.group;
     const int base = sq.base;
     const int r_last = min(rt * kTileRows + kTileRows - 1, rows - 1);
@@ -597,19 +611,19 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
         for (int part = 0; part < W / C; ++part) {
             const int t0 = (step0 + i) * S + part * 16 * C;
             if (!mine || t0 >= wend || t0 + 16 * C <= wbegin) continue;
-            // Operands are read a group ahead of the products that take them: the keys of a chunk, or half of
-            // the values of 32 tokens.
-            bf16x8 f[2][G];
+            // Operands are read a group ahead of the products that take them (where there are the registers for
+            // it): the keys of a chunk, or half of the values of 32 tokens.
+            bf16x8 f[kAhead ? 2 : 1][G];
             const uint8_t* operands = smem[buf][part] + lane * 16;
             auto read = [&](int group) {
 #pragma unroll
-                for (int e = 0; e < G; ++e) f[group & 1][e] = *reinterpret_cast<const bf16x8*>(operands + (group * G + e) * 1024);
+                for (int e = 0; e < G; ++e) f[kAhead ? group & 1 : 0][e] = *reinterpret_cast<const bf16x8*>(operands + (group * G + e) * 1024);
             };
             f32x4 s[NQ][C];
-            read(0);
+            if (kAhead) read(0);
 #pragma unroll
             for (int n = 0; n < C; ++n) {
-                read(n + 1);
+                read(kAhead ? n + 1 : n);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < NQ; ++t) s[t][n] = f32x4{0, 0, 0, 0};
@@ -618,7 +632,7 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
 #pragma unroll
                     for (int t = 0; t < NQ; ++t)
 #pragma unroll
-                        for (int u = 0; u < TERMS; ++u) s[t][n] = mfma(f[n & 1][e], qf[t][e][u], s[t][n]);
+                        for (int u = 0; u < TERMS; ++u) s[t][n] = mfma(f[kAhead ? n & 1 : 0][e], qf[t][e][u], s[t][n]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             uint32_t note = 0;
@@ -710,14 +724,15 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int group = C + 2 * n + half;
-                    if (group + 1 < 2 * C) read(group + 1);
+                    if (!kAhead) read(group);
+                    else if (group + 1 < 2 * C) read(group + 1);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int e = 0; e < G; ++e)
 #pragma unroll
                         for (int t = 0; t < NQ; ++t)
 #pragma unroll
-                            for (int u = 0; u < TERMS; ++u) acc[t][half * G + e] = mfma(f[group & 1][e], pf[t][u], acc[t][half * G + e]);
+                            for (int u = 0; u < TERMS; ++u) acc[t][half * G + e] = mfma(f[kAhead ? group & 1 : 0][e], pf[t][u], acc[t][half * G + e]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }

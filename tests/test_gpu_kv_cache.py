@@ -249,10 +249,13 @@ def test_more_rows_than_tokens_and_rows_behind_the_last_sequence(rows):
     assert (out[n:] == 3.0).all()
     assert not out[: rows[0] - 2].any()
     # of each sequence no more than max_rows
+    # (a call of fewer rows may take another kernel: both are within the bound of the same 64-bit values)
     part = f.attend(q, rows, out=torch.full_like(q, 5.0), max_rows=4)
+    want, bound = ref.attention(q, f.k, f.v, f.lengths, np.cumsum([0] + rows), 0.125, terms=1, dtype=torch.bfloat16)
     at = 0
     for r in rows:
-        assert torch.equal(part[at:at + min(r, 4)], out[at:at + min(r, 4)])
+        done = slice(at, at + min(r, 4))
+        assert (np.abs(ref.f64(part[done]) - want[done]) <= bound[done]).all()
         assert (part[at + min(r, 4):at + r] == 5.0).all()
         at += r
 
