@@ -44,55 +44,138 @@ __device__ __forceinline__ TokenScale token_scale(uint32_t top) {
     return {s, 1.0f / s};
 }
 
-// rne(x / s) of the exact quotient.  x inv is within 2e-5 of it (|x / s| <= 127, two roundings), so
-// away from the halves both round alike; near one the quotient is taken in 64 bits, where it cannot
-// round onto a half that it does not reach (a difference from a half is at least 2^-25 of it).
-__device__ __forceinline__ int quant1(float x, const TokenScale& t) {
-    const float v = x * t.inv;
-    float r = rintf(v);
-    if (fabsf(v - r) > 0.4999f) r = (float)rint((double)x / (double)t.s);
-    return (int)r;
+// rne(x / s) of the exact quotients, as bytes.  One fused multiply-add rounds x inv to an integer in the low
+// bits of 1.5 2^23; inv is within 2^-24 of 1 / s, so x inv is within 127 2^-24 < 1e-5 of the quotient, and
+// unless it lies that near a half h both round alike.  There the sign of x - h s decides, which a fused
+// multiply-add gives exactly; zero is a tie.
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], const TokenScale& t) {
+    constexpr float kInt = 12582912.0f, kNear = 0.49999f;
+    float r[8], d[8], off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        r[e] = fmaf(x[e], t.inv, kInt);
+        d[e] = fmaf(x[e], t.inv, kInt - r[e]);
+        off = fmaxf(off, fabsf(d[e]));
+    }
+    if (off > kNear) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float h = (r[e] - kInt) + copysignf(0.5f, d[e]), past = fmaf(-h, t.s, x[e]);
+            const float q = past == 0.0f ? rintf(h) : h + copysignf(0.5f, past);
+            r[e] = fabsf(d[e]) > kNear ? q + kInt : r[e];
+        }
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float* q = r + 4 * h;
+        const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(q[1]), __float_as_uint(q[0]), 0x0c0c0400u);
+        w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(__float_as_uint(q[3]), __float_as_uint(q[2]), 0x0c0c0400u), a, 0x05040100u);
+    }
+    return make_uint2(w[0], w[1]);
 }
 
-__device__ __forceinline__ uint32_t quant4(const float* x, const TokenScale& t) {
-    return (uint32_t)(quant1(x[0], t) & 255) | (uint32_t)(quant1(x[1], t) & 255) << 8 | (uint32_t)(quant1(x[2], t) & 255) << 16 |
-           (uint32_t)quant1(x[3], t) << 24;
+// Eight values of a row from k on, zeros past K, in two steps, so that the loads of several rows are on their
+// way before the first is used: the load itself, of eight values inside the row (none in a row of fewer),
+// and what they are as floats.
+template <typename T>
+struct Raw8 {
+    typedef T vec __attribute__((ext_vector_type(8)));
+    vec w;
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> ask_row8(const T* row, int k, int K) {
+    Raw8<T> r;
+    if (K >= 8) __builtin_memcpy(&r.w, row + min(k, K - 8), sizeof(r.w));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void take_row8(const Raw8<T>& r, const T* row, int k, int K, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)r.w[e];
+    if (k + 8 > K) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        if (k < K) {
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+                if (k + e < K) v[e] = (float)row[k + e];
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load_row8(const T* row, int k, int K, float (&v)[8]) {
+    take_row8(ask_row8(row, k, K), row, k, K, v);
+}
+__device__ __forceinline__ uint32_t top8(const float (&v)[8], uint32_t top) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    return top;
+}
+// The largest over the wave, the same in every lane: in each row of 16 lanes by exchanges inside vector
+// instructions, then of the four rows.
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true));   // neighbours of a pair
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true));   // pairs of four
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // halves of eight, mirrored
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));  // halves of sixteen
+    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+    const uint32_t b = max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
+    return max(a, b);
 }
 
-// A wave a row.  x's rows start anywhere; q's rows have ldq bytes and are written 8 at a time where
-// that is aligned (VEC), zeros from K to `fill`.
-template <typename T, bool VEC>
+// W waves a row (4, or 1 and four rows a block where rows are short), which keep its first 512 W NV values in
+// registers between the maximum and the rounding; what is behind them is read again.  x's rows start
+// anywhere; q's rows have ldq bytes and are written 8 at a time where that is aligned (VEC), zeros
+// from K to `fill`.
+template <int W, typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) token_quantize_kernel(const T* x, int64_t M, int K, int64_t ldx, int8_t* q, int64_t ldq,
                                                                   int fill, float* scale) {
-    const int64_t m = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    constexpr int NV = 2, STEP = 512 * W;
+    const int64_t m = W == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
     if (m >= M) return;
+    const int t = W == 4 ? threadIdx.x : threadIdx.x & 63;
     const T* row = x + m * ldx;
+    Raw8<T> raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = ask_row8(row, i * STEP + t * 8, K);
     uint32_t top = 0;
-    const int whole = K & ~7;
-    for (int k = lane * 8; k < whole; k += 512) {
-        float v[8];
-        icx::load_f32(row + k, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    for (int k = NV * STEP + t * 8; k < K; k += STEP) {
+        float u[8];
+        load_row8(row, k, K, u);
+        top = top8(u, top);
     }
-    if (whole + lane < K) top = max(top, __float_as_uint((float)row[whole + lane]) & 0x7fffffffu);
+    float v[NV][8];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-    const TokenScale t = token_scale(top);
-    if (lane == 0) scale[m] = t.s;
+    for (int i = 0; i < NV; ++i) {
+        take_row8(raw[i], row, i * STEP + t * 8, K, v[i]);
+        top = top8(v[i], top);
+    }
+    top = wave_top(top);
+    if constexpr (W == 4) {
+        __shared__ uint32_t tops[4];
+        if ((t & 63) == 0) tops[t >> 6] = top;
+        __syncthreads();
+        top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
+    const TokenScale ts = token_scale(top);
+    if (t == 0) scale[m] = ts.s;
     int8_t* out = q + m * ldq;
-    const bool bad = !(t.s == t.s);
-    for (int k = lane * 8; k < (VEC ? fill : K); k += 512) {
-        float v[8];
-        if (k + 8 <= K) icx::load_f32(row + k, v);
-        else
-            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? (float)row[k + e] : 0.0f;
+    const bool bad = !(ts.s == ts.s);
+    auto put = [&](int k, const float (&u)[8]) {
+        if (k >= (VEC ? fill : K)) return;
         uint2 w = make_uint2(0u, 0u);
-        if (!bad) w = make_uint2(quant4(v, t), quant4(v + 4, t));
+        if (!bad) w = quant8(u, ts);
         if (VEC) *reinterpret_cast<uint2*>(out + k) = w;
         else
             for (int e = 0; e < 8 && k + e < K; ++e) out[k + e] = (int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put(i * STEP + t * 8, v[i]);
+    for (int k = NV * STEP + t * 8; k < (VEC ? fill : K); k += STEP) {
+        float u[8];
+        load_row8(row, k, K, u);
+        put(k, u);
     }
 }
 
@@ -112,31 +195,118 @@ struct ProductArgs {
 
 __device__ __forceinline__ float finish(int acc, float xs, float ws, float bias) { return (float)acc * (xs * ws) + bias; }
 
-// 16 tokens by 16 channels a block, K split over its waves (integers: the same sum in any order).
-template <int W, typename T>
-__global__ void __launch_bounds__(64 * W) token_product_small_kernel(ProductArgs g) {
-    __shared__ v4i part[W][64];
+// ---- few tokens ---------------------------------------------------------------------------------
+// 16 TI tokens by 16 channels a block, K split over its eight waves (integers: the same sum in any order).
+// What such a product costs is the walk of the weight, so its loads come first and many at a time: a
+// wave's share of K in groups of U steps of 64, all of a group's fragments asked for before the first is
+// used.  q's fragments come from L2, or with QUANT from LDS, where every block puts all tokens' bytes
+// after asking for its first weights: it quantizes them itself (the same work in every block, under
+// the latency of the weight's walk, in place of a launch before this one), a wave a row.
+constexpr int kSmallWaves = 8;
+
+template <int TI, bool QUANT, typename X, typename T>
+__global__ void __launch_bounds__(64 * kSmallWaves) token_product_small_kernel(ProductArgs g, const X* x, int64_t ldx, int K) {
+    constexpr int W = kSmallWaves, U = 8;
+    extern __shared__ int8_t rows[];  // QUANT: [M][Kp + 16]
+    __shared__ v4i part[W][TI][64];
+    __shared__ float scales[W];
     const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = (int)(blockIdx.x / g.tiles_m) * 16, m0 = (int)(blockIdx.x % g.tiles_m) * 16;
-    const int8_t* a = g.q + (int64_t)min(m0 + lr, g.M - 1) * g.lda + 16 * j;
+    const int n0 = (int)(blockIdx.x / g.tiles_m) * 16, m0 = (int)(blockIdx.x % g.tiles_m) * 16 * TI;
     const int8_t* b = g.w + (int64_t)min(n0 + lr, g.N - 1) * g.Kp + 16 * j;
-    v4i acc = {0, 0, 0, 0};
-    for (int k = wid * 64; k < g.Kp; k += 64 * W)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(a + k), *reinterpret_cast<const v4i*>(b + k), acc, 0,
-                                                    0, 0);
-    part[wid][lane] = acc;
-    __syncthreads();
-    if (wid) return;
+    const int steps = g.Kp / 64, share = (steps + W - 1) / W;
+    const int from = min(steps, wid * share), to = min(steps, from + share);
+    v4i fb[U];
+    auto load_b = [&](int s) {
 #pragma unroll
-    for (int w = 1; w < W; ++w) acc += part[w][lane];
+        for (int u = 0; u < U; ++u) fb[u] = *reinterpret_cast<const v4i*>(b + min(s + u, steps - 1) * 64);
+    };
+    load_b(from);
+    const int ld = g.Kp + 16;  // (rows 16 bytes further apart than whole steps: no two of 8 share banks)
+    if constexpr (QUANT) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (wid < g.M) {
+            constexpr int NV = 8;  // 4096 values of the row stay in registers
+            const X* row = x + wid * ldx;
+            int8_t* out = rows + wid * ld;
+            Raw8<X> raw[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[i] = ask_row8(row, (i * 64 + lane) * 8, K);
+            uint32_t top = 0;
+#pragma unroll 1
+            for (int k = (NV * 64 + lane) * 8; k < K; k += 512) {
+                float u[8];
+                load_row8(row, k, K, u);
+                top = top8(u, top);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float u[8];
+                if (i * 512 >= K) continue;
+                take_row8(raw[i], row, (i * 64 + lane) * 8, K, u);
+                top = top8(u, top);
+            }
+            const TokenScale ts = token_scale(wave_top(top));
+            const bool bad = !(ts.s == ts.s);
+            if (lane == 0) scales[wid] = ts.s;
+            auto put = [&](int k, const float (&u)[8]) {
+                const uint2 w = quant8(u, ts);
+                if (k < g.Kp) *reinterpret_cast<uint2*>(out + k) = bad ? make_uint2(0u, 0u) : w;
+            };
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float u[8];
+                if (i * 512 >= g.Kp) continue;
+                take_row8(raw[i], row, (i * 64 + lane) * 8, K, u);
+                put((i * 64 + lane) * 8, u);
+            }
+#pragma unroll 1
+            for (int k = (NV * 64 + lane) * 8; k < g.Kp; k += 512) {
+                float u[8];
+                load_row8(row, k, K, u);
+                put(k, u);
+            }
+        }
+        __syncthreads();
+    }
+    v4i acc[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) acc[i] = v4i{0, 0, 0, 0};
+    for (int s = from; s < to; s += U) {
+        if (s != from) load_b(s);
+        v4i fa[TI][QUANT ? 1 : U];
+        if constexpr (!QUANT) {
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    fa[i][u] = *reinterpret_cast<const v4i*>(g.q + (int64_t)min(m0 + 16 * i + lr, g.M - 1) * g.lda + min(s + u, steps - 1) * 64 + 16 * j);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // every load of the group before the first product
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s + u >= to) break;
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+                if constexpr (QUANT) fa[i][0] = *reinterpret_cast<const v4i*>(rows + min(lr, g.M - 1) * ld + (s + u) * 64 + 16 * j);
+                acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i][QUANT ? 0 : u], fb[u], acc[i], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) part[wid][i][lane] = acc[i];
+    __syncthreads();
+    if (wid >= TI) return;
+    v4i sum = part[0][wid][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum += part[w][wid][lane];
     const int n = n0 + lr;
     if (n >= g.N) return;
     const float ws = g.ws[n], bias = g.bias ? g.bias[n] : 0.0f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int m = m0 + 4 * j + r;
-        if (m < g.M) reinterpret_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = (T)finish(acc[r], g.xs[m], ws, bias);
+        const int m = m0 + 16 * wid + 4 * j + r;
+        if (m < g.M) reinterpret_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = (T)finish(sum[r], QUANT ? scales[m] : g.xs[m], ws, bias);
     }
 }
 
@@ -197,21 +367,22 @@ __device__ __forceinline__ void tile_of(const ProductArgs& g, int& tm, int& tn) 
 
 constexpr int kBig = 256, kStep = 128;
 
-// 16 channels of one token from n on.
-template <typename T>
-__device__ __forceinline__ void store16(T* row, int n, int N, bool wide, const float (&v)[16]) {
-    if (wide && n + 16 <= N) {
-        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+// C channels of one token from n on.
+template <int C, typename T>
+__device__ __forceinline__ void store_channels(T* row, int n, int N, bool wide, const float (&v)[C]) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (wide && n + C <= N) {
+        typedef T vec __attribute__((ext_vector_type(V)));
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T); ++i) {
+        for (int i = 0; i < C / V; ++i) {
             vec w;
 #pragma unroll
-            for (int e = 0; e < 16 / (int)sizeof(T); ++e) w[e] = (T)v[i * (16 / sizeof(T)) + e];
-            *reinterpret_cast<vec*>(row + n + i * (16 / sizeof(T))) = w;
+            for (int e = 0; e < V; ++e) w[e] = (T)v[i * V + e];
+            *reinterpret_cast<vec*>(row + n + i * V) = w;
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+        for (int e = 0; e < C; ++e)
             if (n + e < N) row[n + e] = (T)v[e];
     }
 }
@@ -334,7 +505,108 @@ __global__ void __launch_bounds__(512, 2) token_product_big_kernel(ProductArgs g
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[4 * t + r] = finish(acc[i][t][r], xs, ws[4 * t + r], bias[4 * t + r]);
-        store16(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, wide, v);
+        store_channels<16>(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, wide, v);
+    }
+}
+
+// ---- between them: tiles of 64 x 64 and 128 x 128 ---------------------------------------------------
+// Four waves, 2 x 2, each half of either side; NS steps of 128 bytes of K stand in LDS, NS - 1 of them on
+// their way, one barrier a step: past it step kt has landed (its copies are waited for by the count of
+// those issued after them) and the buffer that step kt - 1 was read from takes the copies of step
+// kt + NS - 1.  Channels are laid out over a wave's tiles as above, a lane's results 4 TN consecutive ones.
+template <int N>
+__device__ __forceinline__ void wait_copies_but() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+template <int B, int NS, typename T>
+__global__ void __launch_bounds__(256) token_product_tile_kernel(ProductArgs g) {
+    constexpr int TN = B / 32;  // tiles of 16 on either side of a wave's B / 2
+    constexpr int P = B / 32;   // copies of each operand a wave and step
+    __shared__ __attribute__((aligned(1024))) int8_t smem[NS][2 * B * kStep];
+    int tm, tn;
+    tile_of(g, tm, tn);
+    const int m0 = tm * B, n0 = tn * B;
+    const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wid >> 1, wn = wid & 1;
+    // bits 1 and the next two of those that tell the 16 rows of a fragment apart
+    auto key = [&](int row) { return ((row >> 1) & 1) | ((row / (4 * TN)) & 3) << 1; };
+
+    const int8_t* qa = g.q + (int64_t)m0 * g.lda;
+    const int8_t* wa = g.w + (int64_t)n0 * g.Kp;
+    uint32_t oq[P], ow[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int row = (wid * P + i) * 8 + (lane >> 3);
+        oq[i] = (uint32_t)((int64_t)min(row, g.M - 1 - m0) * g.lda + 16 * ((lane & 7) ^ token_key(row)));
+        ow[i] = (uint32_t)((int64_t)min(row, g.N - 1 - n0) * g.Kp + 16 * ((lane & 7) ^ key(row)));
+    }
+    const uint32_t lds = lds_address(smem) + wid * P * 8 * kStep;
+    const int KT = g.Kp / kStep;
+    auto copy = [&](int kt) {
+        const uint32_t to = lds + (uint32_t)(kt % NS) * (2 * B * kStep);
+        const int k = min(kt, KT - 1) * kStep;  // past the end: the last step again, into a buffer that nobody reads
+#pragma unroll
+        for (int i = 0; i < P; ++i) copy_to_lds(qa + k, oq[i], to + i * 8 * kStep);
+#pragma unroll
+        for (int i = 0; i < P; ++i) copy_to_lds(wa + k, ow[i], to + B * kStep + i * 8 * kStep);
+    };
+    v4i acc[TN][TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int t = 0; t < TN; ++t) acc[i][t] = v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) copy(s);
+    for (int kt = 0; kt < KT; ++kt) {
+        wait_copies_but<2 * P * (NS - 2)>();
+        barrier();
+        copy(kt + NS - 1);
+        const int8_t* a = smem[kt % NS];
+        const int8_t* b = a + B * kStep;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            v4i fq[TN], fw[TN];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                const int row = wm * (B / 2) + i * 16 + lr;
+                fq[i] = *reinterpret_cast<const v4i*>(a + row * kStep + 16 * ((4 * k + j) ^ token_key(row)));
+            }
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const int row = wn * (B / 2) + (lr >> 2) * 4 * TN + t * 4 + (lr & 3);
+                fw[t] = *reinterpret_cast<const v4i*>(b + row * kStep + 16 * ((4 * k + j) ^ key(row)));
+            }
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int t = 0; t < TN; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fq[i], acc[i][t], 0, 0, 0);
+        }
+    }
+    wait_copies();  // (those past the end)
+
+    constexpr int C = 4 * TN;  // channels of a lane
+    const int n = n0 + wn * (B / 2) + C * j;
+    float ws[C], bias[C];
+#pragma unroll
+    for (int e = 0; e < C; ++e) {
+        const int c = min(n + e, g.N - 1);
+        ws[e] = g.ws[c];
+        bias[e] = g.bias ? g.bias[c] : 0.0f;
+    }
+    const bool wide = (g.ldy * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const int m = m0 + wm * (B / 2) + i * 16 + lr;
+        if (m >= g.M) continue;
+        const float xs = g.xs[m];
+        float v[C];
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[4 * t + r] = finish(acc[i][t][r], xs, ws[4 * t + r], bias[4 * t + r]);
+        store_channels<C>(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, wide, v);
     }
 }
 
@@ -347,11 +619,13 @@ __global__ void __launch_bounds__(kThreads) token_pad_kernel(const int8_t* q, in
 int quantize(hipStream_t s, const void* x, int dtype, size_t M, size_t K, int64_t ldx, int8_t* q, size_t ldq, size_t fill,
              float* scale) {
     const bool vec = ldq % 8 == 0 && fill % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-    const unsigned blocks = (unsigned)icx::cdiv(M, kThreads / 64);
+    const bool wide = K > 1024;
+    const unsigned blocks = (unsigned)(wide ? M : icx::cdiv(M, kThreads / 64));
     return icx::with_float_type(dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (vec) token_quantize_kernel<T, true><<<blocks, kThreads, 0, s>>>((const T*)x, M, (int)K, ldx, q, ldq, (int)fill, scale);
-        else token_quantize_kernel<T, false><<<blocks, kThreads, 0, s>>>((const T*)x, M, (int)K, ldx, q, ldq, (int)fill, scale);
+        auto launch = [&](auto kernel) { kernel<<<blocks, kThreads, 0, s>>>((const T*)x, M, (int)K, ldx, q, ldq, (int)fill, scale); };
+        if (wide) vec ? launch(token_quantize_kernel<4, T, true>) : launch(token_quantize_kernel<4, T, false>);
+        else vec ? launch(token_quantize_kernel<1, T, true>) : launch(token_quantize_kernel<1, T, false>);
         ICX_LAUNCH_CHECK("token_quantize_kernel");
         return ICX_OK;
     });
@@ -365,6 +639,23 @@ Workspace workspace(size_t M, size_t K, int x_dtype) {
     const size_t q = icx::align_up(M * padded(K), 256);
     return {q, q + (x_dtype == ICX_I8 ? 0 : 4 * M)};
 }
+
+// Which kernel takes an M x N product, and its tile.
+struct Form {
+    int kind;  // 256, 128 or 64 for a tile of that, else 16-token tiles of token_product_small_kernel
+    size_t tile_m, tile_n;
+};
+Form form_of(size_t M, size_t N) {
+    const size_t cus = (size_t)icx::num_cus();
+    if (M <= 16) return {1, 16, 16};
+    if (M <= 32) return {2, 32, 16};
+    if (M <= 64) return {4, 64, 16};
+    if (icx::cdiv(M, 256) * icx::cdiv(N, 256) * 4 >= 3 * cus) return {256, 256, 256};
+    if (icx::cdiv(M, 128) * icx::cdiv(N, 128) >= cus) return {128, 128, 128};
+    return {64, 64, 64};
+}
+// Tokens that every block of the product quantizes for itself, and the LDS that they may take.
+constexpr size_t kFusedTokens = kSmallWaves, kFusedBytes = 128 * 1024;
 
 // The sums stay within 32 bits: |w|, |q| <= 128.
 constexpr size_t kMaxK = 131071;
@@ -435,6 +726,32 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, L.total, ws_bytes);
     const hipStream_t s = (hipStream_t)stream;
     ProductArgs g{};
+    g.w = packed;
+    g.ws = w_scale;
+    g.bias = bias;
+    g.y = y;
+    g.ldy = y_stride;
+    g.M = (int)M;
+    g.N = (int)N;
+    g.Kp = (int)padded(K);
+    const Form form = form_of(M, N);
+    g.tiles_m = (int)icx::cdiv(M, form.tile_m);
+    g.tiles_n = (int)icx::cdiv(N, form.tile_n);
+    if ((uint64_t)g.tiles_m * g.tiles_n > 0x7fffff)
+        ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu x %zu outputs are too many for a launch", who, M, N);
+    const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n);
+    const size_t lds = M * (padded(K) + 16);
+    if (own && M <= kFusedTokens && lds <= kFusedBytes) {
+        return icx::with_float_type(x_dtype, [&](auto* xt) -> int {
+            using X = std::remove_pointer_t<decltype(xt)>;
+            return icx::with_float_type(y_dtype, [&](auto* yt) -> int {
+                using T = std::remove_pointer_t<decltype(yt)>;
+                token_product_small_kernel<1, true, X, T><<<blocks, 64 * kSmallWaves, lds, s>>>(g, (const X*)x, x_stride, (int)K);
+                ICX_LAUNCH_CHECK("token_product_small_kernel");
+                return ICX_OK;
+            });
+        });
+    }
     g.q = (const int8_t*)x;
     g.lda = x_stride;
     g.xs = x_scale;
@@ -451,30 +768,18 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
         g.q = (const int8_t*)ws;
         g.lda = (int64_t)padded(K);
     }
-    g.w = packed;
-    g.ws = w_scale;
-    g.bias = bias;
-    g.y = y;
-    g.ldy = y_stride;
-    g.M = (int)M;
-    g.N = (int)N;
-    g.Kp = (int)padded(K);
-    const bool big = M >= 1024 && icx::cdiv(M, kBig) * icx::cdiv(N, kBig) >= 64;
-    const size_t tile = big ? kBig : 16;
-    g.tiles_m = (int)icx::cdiv(M, tile);
-    g.tiles_n = (int)icx::cdiv(N, tile);
-    if ((uint64_t)g.tiles_m * g.tiles_n * 256 > 0xffffffffull)
-        ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu x %zu outputs are too many for a launch", who, M, N);
-    const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n);
     return icx::with_float_type(y_dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (big) {
-            token_product_big_kernel<T><<<blocks, 512, 0, s>>>(g);
-            ICX_LAUNCH_CHECK("token_product_big_kernel");
-            return ICX_OK;
+        const int8_t* none = nullptr;
+        switch (form.kind) {
+            case 256: token_product_big_kernel<T><<<blocks, 512, 0, s>>>(g); break;
+            case 128: token_product_tile_kernel<128, 2, T><<<blocks, 256, 0, s>>>(g); break;
+            case 64: token_product_tile_kernel<64, 3, T><<<blocks, 256, 0, s>>>(g); break;
+            case 4: token_product_small_kernel<4, false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
+            case 2: token_product_small_kernel<2, false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
+            default: token_product_small_kernel<1, false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
         }
-        token_product_small_kernel<4, T><<<blocks, 256, 0, s>>>(g);
-        ICX_LAUNCH_CHECK("token_product_small_kernel");
+        ICX_LAUNCH_CHECK("token_product");
         return ICX_OK;
     });
 }
