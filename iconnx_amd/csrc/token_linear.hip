@@ -631,15 +631,6 @@ int quantize(hipStream_t s, const void* x, int dtype, size_t M, size_t K, int64_
     });
 }
 
-// q [M, Kp] and, behind it, the scales (Int8 tokens: room for rows that have to be padded).
-struct Workspace {
-    size_t scale_off, total;
-};
-Workspace workspace(size_t M, size_t K, int x_dtype) {
-    const size_t q = icx::align_up(M * padded(K), 256);
-    return {q, q + (x_dtype == ICX_I8 ? 0 : 4 * M)};
-}
-
 // Which kernel takes an M x N product, and its tile.
 struct Form {
     int kind;  // 256, 128 or 64 for a tile of that, else 16-token tiles of token_product_small_kernel
@@ -656,6 +647,18 @@ Form form_of(size_t M, size_t N) {
 }
 // Tokens that every block of the product quantizes for itself, and the LDS that they may take.
 constexpr size_t kFusedTokens = kSmallWaves, kFusedBytes = 128 * 1024;
+inline size_t fused_lds(size_t M, size_t K) { return M * (padded(K) + 16); }
+inline bool fused(size_t M, size_t K) { return M <= kFusedTokens && fused_lds(M, K) <= kFusedBytes; }
+
+// q [M, Kp] and, behind it, the scales (Int8 tokens: room for rows that have to be padded).
+struct Workspace {
+    size_t scale_off, total;
+};
+Workspace workspace(size_t M, size_t K, int x_dtype) {
+    if (x_dtype != ICX_I8 && fused(M, K)) return {0, 0};
+    const size_t q = icx::align_up(M * padded(K), 256);
+    return {q, q + (x_dtype == ICX_I8 ? 0 : 4 * M)};
+}
 
 // The sums stay within 32 bits: |w|, |q| <= 128.
 constexpr size_t kMaxK = 131071;
@@ -722,7 +725,7 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
     if (!icx::aligned16(packed)) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: the packed weight must be 16-byte aligned", who);
     const Workspace L = workspace(M, K, x_dtype);
     const bool pad = !own && (K % kAlignK || x_stride % 16 || !icx::aligned16(x));
-    if ((own || pad) && (!ws || ws_bytes < L.total))
+    if ((own || pad) && L.total && (!ws || ws_bytes < L.total))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, L.total, ws_bytes);
     const hipStream_t s = (hipStream_t)stream;
     ProductArgs g{};
@@ -740,8 +743,8 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
     if ((uint64_t)g.tiles_m * g.tiles_n > 0x7fffff)
         ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu x %zu outputs are too many for a launch", who, M, N);
     const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n);
-    const size_t lds = M * (padded(K) + 16);
-    if (own && M <= kFusedTokens && lds <= kFusedBytes) {
+    if (own && fused(M, K)) {
+        const size_t lds = fused_lds(M, K);
         return icx::with_float_type(x_dtype, [&](auto* xt) -> int {
             using X = std::remove_pointer_t<decltype(xt)>;
             return icx::with_float_type(y_dtype, [&](auto* yt) -> int {

@@ -581,32 +581,37 @@ def gpu_attention(q, k, v, heads, scale, scale_div=True, scale_q=False):
 # ---------------------------------------------------------------------------------------
 _FLOAT = {torch.float32: ICX_F32, torch.float16: ICX_F16, torch.bfloat16: ICX_BF16}
 _INDEX = {torch.int32: ICX_I32, torch.int64: ICX_I64}
+_I8, _BF16, _F16 = torch.int8, torch.bfloat16, torch.float16
 
 
-def _float_code(t, who):
-    code = _FLOAT.get(t.dtype if isinstance(t, torch.Tensor) else t)
+def _float_code(dtype, who):
+    code = _FLOAT.get(dtype)
     if code is None:
-        raise IconnxError(ERR_DTYPE, "%s: dtype %s unsupported (must be Float32, Float16 or BFloat16)"
-                          % (who, _name(t.dtype if isinstance(t, torch.Tensor) else t)))
+        raise IconnxError(ERR_DTYPE, "%s: dtype %s unsupported (must be Float32, Float16 or BFloat16)" % (who, _name(dtype)))
     return code
 
 
-def _one_device(who, *ts):
+def _here():
+    return _cur_device() if _cur_device else torch.cuda.current_device()
+
+
+def _on_device(who, here, *ts):
     """Every tensor on the current device: the kernels run there, on its current stream."""
-    _require_cuda(*ts)
-    here = _cur_device() if _cur_device else torch.cuda.current_device()
     for t in ts:
         if t is not None and t.get_device() != here:
+            _require_cuda(t)
             raise IconnxError(ERR_INVALID, "%s: a tensor is on device %d, the current one is %d" % (who, t.get_device(), here))
 
 
 def _rows(x):
-    """x [..., K] as rows: (rows, K, row stride, the tensor that holds them)."""
-    if x.dim() == 2 and x.stride(1) == 1:
-        return x.shape[0], x.shape[1], x.stride(0), x
+    """x [..., K] as rows: (rows, row stride, the tensor that holds them)."""
+    if x.dim() == 2:
+        ld, one = x.stride()
+        if one == 1:
+            return x.shape[0], ld, x
     x = _dense(x)
     K = x.shape[-1]
-    return (x.numel() // K if K else 0), K, K, x
+    return (x.numel() // K if K else 0), K, x
 
 
 class TokenWeight:
@@ -615,20 +620,22 @@ class TokenWeight:
 
     def __init__(self, b, scale):
         who = "TokenWeight"
-        if b.dtype != torch.int8:
+        if b.dtype != _I8:
             raise IconnxError(ERR_DTYPE, "%s: the weight must be Int8, got %s" % (who, _name(b.dtype)))
         if scale.dtype != _F32:
             raise IconnxError(ERR_DTYPE, "%s: the scale must be Float32, got %s" % (who, _name(scale.dtype)))
         if b.dim() != 2 or tuple(scale.shape) != (b.shape[1],):
             raise IconnxError(ERR_SHAPE, "%s: a weight [K, N] and a scale [N] (got %s and %s)"
                               % (who, list(b.shape), list(scale.shape)))
-        _one_device(who, b, scale)
+        _require_cuda(b, scale)
+        _on_device(who, _here(), b, scale)
         b = _dense(b)
         self.K, self.N = b.shape
         self.scale = scale.contiguous()
         L = lib()
-        self.packed = _empty(L.icx_token_weight_bytes(self.K, self.N), dtype=torch.int8, device=b.device)
+        self.packed = _empty(L.icx_token_weight_bytes(self.K, self.N), dtype=_I8, device=b.device)
         check(L.icx_pack_token_weight(_stream(), b.data_ptr(), self.K, self.N, self.packed.data_ptr()))
+        self._device, self._ws = self.packed.get_device(), {}
 
     @property
     def shape(self):
@@ -640,14 +647,16 @@ def gpu_quantize_tokens(x):
     max(max|x| / 127, 2^-126) and q = x / scale rounded to nearest even.  A token that is not finite
     throughout has the scale NaN and zeros."""
     who = "QuantizeTokens"
-    code = _float_code(x, who)
-    if x.dim() < 1:
+    code = _float_code(x.dtype, who)
+    shape = x.shape
+    if not shape:
         raise IconnxError(ERR_SHAPE, "%s: x has no tokens (shape [])" % who)
-    _one_device(who, x)
-    M, K, ld, x = _rows(x)
-    q = _empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = _empty(x.shape[:-1], dtype=_F32, device=x.device)
-    check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, K, ld, q.data_ptr(), scale.data_ptr()))
+    _on_device(who, _here(), x)
+    M, ld, x = _rows(x)
+    dev = x.device
+    q = _empty(shape, dtype=_I8, device=dev)
+    scale = _empty(shape[:-1], dtype=_F32, device=dev)
+    check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, shape[-1], ld, q.data_ptr(), scale.data_ptr()))
     return q, scale
 
 
@@ -658,37 +667,48 @@ def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
     who = "TokenQLinear"
     if not isinstance(w, TokenWeight):
         raise IconnxError(ERR_INVALID, "%s: the weight must be a TokenWeight" % who)
-    if x.dtype == torch.int8:
+    shape, K, N, here = x.shape, w.K, w.N, _here()
+    if x.dtype == _I8:
         code, yt = ICX_I8, dtype or _F32
         if x_scale is None:
             raise IconnxError(ERR_INVALID, "%s: Int8 tokens come with their scales" % who)
-        if x_scale.dtype != _F32 or x_scale.shape != x.shape[:-1]:
+        if x_scale.dtype != _F32 or x_scale.shape != shape[:-1]:
             raise IconnxError(ERR_SHAPE, "%s: x_scale must be Float32 %s, got %s %s"
-                              % (who, list(x.shape[:-1]), _name(x_scale.dtype), list(x_scale.shape)))
+                              % (who, list(shape[:-1]), _name(x_scale.dtype), list(x_scale.shape)))
+        _on_device(who, here, x_scale)
+        x_scale = _dense(x_scale)
     else:
-        code, yt = _float_code(x, who), dtype or x.dtype
+        code, yt = _float_code(x.dtype, who), dtype or x.dtype
         if x_scale is not None:
             raise IconnxError(ERR_INVALID, "%s: x_scale goes with Int8 tokens" % who)
-    ycode = _float_code(yt, who)
-    if x.dim() < 1 or x.shape[-1] != w.K:
-        raise IconnxError(ERR_SHAPE, "%s: K mismatch — x is %s, the weight [%d,%d]" % (who, list(x.shape), w.K, w.N))
+    ycode = code if yt == x.dtype else _float_code(yt, who)
+    if not shape or shape[-1] != K:
+        raise IconnxError(ERR_SHAPE, "%s: K mismatch — x is %s, the weight [%d,%d]" % (who, list(shape), K, N))
+    if x.get_device() != here or w._device != here:
+        _on_device(who, here, x, w.packed)
     if bias is not None:
-        if bias.dtype != _F32 or tuple(bias.shape) != (w.N,):
-            raise IconnxError(ERR_SHAPE, "%s: bias must be Float32 [%d], got %s %s" % (who, w.N, _name(bias.dtype), list(bias.shape)))
+        if bias.dtype != _F32 or bias.dim() != 1 or bias.shape[0] != N:
+            raise IconnxError(ERR_SHAPE, "%s: bias must be Float32 [%d], got %s %s" % (who, N, _name(bias.dtype), list(bias.shape)))
+        _on_device(who, here, bias)
         bias = _dense(bias)
-    shape = x.shape[:-1] + (w.N,)
-    if out is not None and (out.dtype != yt or out.shape != shape or not out.is_contiguous()):
-        raise IconnxError(ERR_SHAPE, "%s: out must be a contiguous %s %s" % (who, _name(yt), list(shape)))
-    _one_device(who, x, x_scale, bias, out, w.packed)
-    M, K, ld, x = _rows(x)
-    if x_scale is not None:
-        x_scale = _dense(x_scale)
-    y = out if out is not None else _empty(shape, dtype=yt, device=x.device)
+    oshape = shape[:-1] + (N,)
+    if out is not None:
+        if out.dtype != yt or out.shape != oshape or not out.is_contiguous():
+            raise IconnxError(ERR_SHAPE, "%s: out must be a contiguous %s %s" % (who, _name(yt), list(oshape)))
+        _on_device(who, here, out)
+    M, ld, x = _rows(x)
     L = lib()
-    nws = L.icx_token_qlinear_workspace_size(M, K, w.N, code)
-    ws = _workspace(nws, x.device)
-    check(L.icx_token_qlinear(_stream(), x.data_ptr(), code, ld, _p(x_scale), M, K, w.N, w.packed.data_ptr(), w.scale.data_ptr(),
-                              _p(bias), y.data_ptr(), ycode, w.N, ws.data_ptr(), nws or 1))
+    nws = w._ws.get((M, code))
+    if nws is None:
+        if len(w._ws) > 4096:  # (a size for each number of tokens that came by)
+            w._ws.clear()
+        nws = w._ws[(M, code)] = L.icx_token_qlinear_workspace_size(M, K, N, code)
+    dev = x.device
+    y = _empty(oshape, dtype=yt, device=dev) if out is None else out
+    ws = _empty(nws, dtype=_U8, device=dev) if nws else None
+    check(L.icx_token_qlinear(_stream(), x.data_ptr(), code, ld, None if x_scale is None else x_scale.data_ptr(), M, K, N,
+                              w.packed.data_ptr(), w.scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+                              ycode, N, None if ws is None else ws.data_ptr(), nws))
     return y
 
 
@@ -707,46 +727,58 @@ class KvCache:
         self.data = torch.zeros(n, dtype=_U8, device=device)
         _require_cuda(self.data)
         self._desc.data = self.data.data_ptr()
+        self._device, self._heads = self.data.get_device(), (kv_heads, head_size)
         self._as_parameter_ = ctypes.addressof(self._desc)  # what a pointer argument takes when given the cache
 
 
-def _slots(slots, who):
+def _check_slots(slots, who):
     code = _INDEX.get(slots.dtype)
     if code is None:
         raise IconnxError(ERR_DTYPE, "%s: slots must be Int64 or Int32, got %s" % (who, _name(slots.dtype)))
     if slots.dim() != 1:
         raise IconnxError(ERR_SHAPE, "%s: slots must be 1-D (got %s)" % (who, list(slots.shape)))
-    return code, _dense(slots)
+    return code
 
 
 def gpu_kv_cache_write(cache, k, v, slots):
     """Quantizes k and v [tokens, kv_heads, head_size] (any strides with dense heads) into the cache's
     ``slots`` [tokens]; a slot outside the cache, as -1, is passed over."""
     who = "KvCacheWrite"
-    code = _float_code(k, who)
+    code = _float_code(k.dtype, who)
     if v.dtype != k.dtype:
         raise IconnxError(ERR_DTYPE, "%s: k is %s, v %s" % (who, _name(k.dtype), _name(v.dtype)))
-    shape = (slots.shape[0] if slots.dim() else -1, cache.kv_heads, cache.head_size)
-    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+    sc = _check_slots(slots, who)
+    n = slots.shape[0]
+    shape = (n,) + cache._heads
+    if k.shape != shape or v.shape != shape:
         raise IconnxError(ERR_SHAPE, "%s: k and v must be %s (got %s and %s)" % (who, list(shape), list(k.shape), list(v.shape)))
-    sc, slots = _slots(slots, who)
-    _one_device(who, k, v, slots, cache.data)
-    k = k if k.stride(2) == 1 else k.contiguous()
-    v = v if v.stride(2) == 1 else v.contiguous()
-    check(lib().icx_kv_cache_write(_stream(), cache, k.data_ptr(), v.data_ptr(), code, shape[0], k.stride(0), k.stride(1), v.stride(0),
-                                   v.stride(1), slots.data_ptr(), sc))
+    here = _here()
+    _on_device(who, here, k, v, slots, None if cache._device == here else cache.data)
+    slots = _dense(slots)
+    kt, kh, one = k.stride()
+    if one != 1:
+        k = k.contiguous()
+        kt, kh, _ = k.stride()
+    vt, vh, one = v.stride()
+    if one != 1:
+        v = v.contiguous()
+        vt, vh, _ = v.stride()
+    check(lib().icx_kv_cache_write(_stream(), cache, k.data_ptr(), v.data_ptr(), code, n, kt, kh, vt, vh, slots.data_ptr(), sc))
 
 
 def gpu_kv_cache_read(cache, slots, dtype=torch.float32):
     """(k, v) [tokens, kv_heads, head_size] that the cache holds at ``slots``; zeros for a slot outside it."""
     who = "KvCacheRead"
     code = _float_code(dtype, who)
-    sc, slots = _slots(slots, who)
-    _one_device(who, slots, cache.data)
-    shape = (slots.shape[0], cache.kv_heads, cache.head_size)
-    k = _empty(shape, dtype=dtype, device=slots.device)
-    v = _empty(shape, dtype=dtype, device=slots.device)
-    check(lib().icx_kv_cache_read(_stream(), cache, slots.data_ptr(), sc, shape[0], k.data_ptr(), v.data_ptr(), code))
+    sc = _check_slots(slots, who)
+    here = _here()
+    _on_device(who, here, slots, None if cache._device == here else cache.data)
+    slots = _dense(slots)
+    n, dev = slots.shape[0], slots.device
+    shape = (n,) + cache._heads
+    k = _empty(shape, dtype=dtype, device=dev)
+    v = _empty(shape, dtype=dtype, device=dev)
+    check(lib().icx_kv_cache_read(_stream(), cache, slots.data_ptr(), sc, n, k.data_ptr(), v.data_ptr(), code))
     return k, v
 
 
@@ -766,45 +798,51 @@ def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_row
     (head_size ** -0.5), through softcap tanh(. / ``softcap``) if that is given, plus ``slopes``[head]
     (j - p), float32.  A row that sees no token is zero; rows of ``out`` past q_starts[batch] keep what they held."""
     who = "KvCacheAttention"
-    code = _float_code(q, who)
-    if q.dim() != 3 or q.shape[2] != cache.head_size:
-        raise IconnxError(ERR_SHAPE, "%s: q must be [rows, heads, %d] (got %s)" % (who, cache.head_size, list(q.shape)))
-    i32 = torch.int32
-    if page_table.dtype != i32 or lengths.dtype != i32 or (q_starts is not None and q_starts.dtype != i32):
+    code = _float_code(q.dtype, who)
+    shape, D = q.shape, cache.head_size
+    if len(shape) != 3 or shape[2] != D:
+        raise IconnxError(ERR_SHAPE, "%s: q must be [rows, heads, %d] (got %s)" % (who, D, list(shape)))
+    if page_table.dtype != _I32 or lengths.dtype != _I32 or (q_starts is not None and q_starts.dtype != _I32):
         raise IconnxError(ERR_DTYPE, "%s: page_table, lengths and q_starts must be Int32" % who)
-    batch = lengths.shape[0] if lengths.dim() == 1 else -1
-    if page_table.dim() != 2 or page_table.shape[0] != batch or (q_starts is not None and tuple(q_starts.shape) != (batch + 1,)):
+    ts, ls = page_table.shape, lengths.shape
+    if len(ls) != 1 or len(ts) != 2 or ts[0] != ls[0] or (q_starts is not None and tuple(q_starts.shape) != (ls[0] + 1,)):
         raise IconnxError(ERR_SHAPE, "%s: page_table [batch, width], lengths [batch], q_starts [batch + 1] (got %s, %s, %s)"
-                          % (who, list(page_table.shape), list(lengths.shape), None if q_starts is None else list(q_starts.shape)))
-    rows, heads, _ = q.shape
+                          % (who, list(ts), list(ls), None if q_starts is None else list(q_starts.shape)))
+    rows, heads, _ = shape
     if slopes is not None:
         if slopes.dtype != _F32 or tuple(slopes.shape) != (heads,):
             raise IconnxError(ERR_SHAPE, "%s: slopes must be Float32 [%d], got %s %s"
                               % (who, heads, _name(slopes.dtype), list(slopes.shape)))
         slopes = _dense(slopes)
-    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1):
-        raise IconnxError(ERR_SHAPE, "%s: out must be a %s %s with dense heads" % (who, _name(q.dtype), list(q.shape)))
-    _one_device(who, q, page_table, lengths, q_starts, slopes, out, cache.data)
-    if q.stride(2) != 1:
+    if out is not None and (out.dtype != q.dtype or out.shape != shape or out.stride(2) != 1):
+        raise IconnxError(ERR_SHAPE, "%s: out must be a %s %s with dense heads" % (who, _name(q.dtype), list(shape)))
+    here = _here()
+    _on_device(who, here, q, page_table, lengths, q_starts, slopes, out, None if cache._device == here else cache.data)
+    qr, qh, one = q.stride()
+    if one != 1:
         q = q.contiguous()
-    if page_table.stride(1) != 1:
+        qr, qh, _ = q.stride()
+    tr, one = page_table.stride()
+    if one != 1:
         page_table = page_table.contiguous()
+        tr = ts[1]
     lengths = _dense(lengths)
     if q_starts is not None:
         q_starts = _dense(q_starts)
+    dev = q.device
     if out is None:
-        out = _empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _empty(shape, dtype=q.dtype, device=dev)
+    orow, oh, _ = out.stride()
     if max_rows is None:
         max_rows = 1 if q_starts is None else rows
     args = _ATTENTION_PACK.pack(
-        q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), page_table.data_ptr(),
-        page_table.stride(0), lengths.data_ptr(), 0 if q_starts is None else q_starts.data_ptr(),
-        0 if slopes is None else slopes.data_ptr(), code, rows, batch, heads, max_rows, page_table.shape[1],
-        cache.head_size ** -0.5 if scale is None else scale, softcap, window, 1 if causal else 0)
+        q.data_ptr(), out.data_ptr(), qr, qh, orow, oh, page_table.data_ptr(), tr, lengths.data_ptr(),
+        0 if q_starts is None else q_starts.data_ptr(), 0 if slopes is None else slopes.data_ptr(), code, rows, ls[0], heads,
+        max_rows, ts[1], D ** -0.5 if scale is None else scale, softcap, window, 1 if causal else 0)
     L = lib()
     nws = L.icx_kv_cache_attention_workspace_size(cache, args)
-    ws = _workspace(nws, q.device)
-    check(L.icx_kv_cache_attention(_stream(), cache, args, ws.data_ptr(), nws))
+    ws = _empty(nws, dtype=_U8, device=dev) if nws else None
+    check(L.icx_kv_cache_attention(_stream(), cache, args, None if ws is None else ws.data_ptr(), nws))
     return out
 
 

@@ -348,7 +348,7 @@ int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dtype, size_t 
                         float* scale);
 /* x: ICX_I8 with x_scale [M] (icx_quantize_tokens' outputs, for several products over one input), or a
  * float type with x_scale NULL, quantized on the way.  y [M, N] of y_dtype, row stride y_stride;
- * bias [N] f32 or NULL. */
+ * bias [N] f32 or NULL.  Few tokens need no workspace (0). */
 size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N, int x_dtype);
 int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype, int64_t x_stride, const float* x_scale, size_t M,
                       size_t K, size_t N, const int8_t* packed, const float* w_scale, const float* bias, void* y, int y_dtype,
