@@ -196,7 +196,7 @@ struct ProductArgs {
 __device__ __forceinline__ float finish(int acc, float xs, float ws, float bias) { return (float)acc * (xs * ws) + bias; }
 
 // ---- few tokens ---------------------------------------------------------------------------------
-// 16 TI tokens by 16 channels a block, K split over its eight waves (integers: the same sum in any order).
+// 16 tokens by 16 channels a block, K split over its eight waves (integers: the same sum in any order).
 // What such a product costs is the walk of the weight, so its loads come first and many at a time: a
 // wave's share of K in groups of U steps of 64, all of a group's fragments asked for before the first is
 // used.  q's fragments come from L2, or with QUANT from LDS, where every block puts all tokens' bytes
@@ -204,15 +204,15 @@ __device__ __forceinline__ float finish(int acc, float xs, float ws, float bias)
 // the latency of the weight's walk, in place of a launch before this one), a wave a row.
 constexpr int kSmallWaves = 8;
 
-template <int TI, bool QUANT, typename X, typename T>
+template <bool QUANT, typename X, typename T>
 __global__ void __launch_bounds__(64 * kSmallWaves) token_product_small_kernel(ProductArgs g, const X* x, int64_t ldx, int K) {
     constexpr int W = kSmallWaves, U = 8;
     extern __shared__ int8_t rows[];  // QUANT: [M][Kp + 16]
-    __shared__ v4i part[W][TI][64];
+    __shared__ v4i part[W][64];
     __shared__ float scales[W];
     const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = (int)(blockIdx.x / g.tiles_m) * 16, m0 = (int)(blockIdx.x % g.tiles_m) * 16 * TI;
+    const int n0 = (int)(blockIdx.x / g.tiles_m) * 16, m0 = (int)(blockIdx.x % g.tiles_m) * 16;
     const int8_t* b = g.w + (int64_t)min(n0 + lr, g.N - 1) * g.Kp + 16 * j;
     const int steps = g.Kp / 64, share = (steps + W - 1) / W;
     const int from = min(steps, wid * share), to = min(steps, from + share);
@@ -269,44 +269,35 @@ __global__ void __launch_bounds__(64 * kSmallWaves) token_product_small_kernel(P
         }
         __syncthreads();
     }
-    v4i acc[TI];
-#pragma unroll
-    for (int i = 0; i < TI; ++i) acc[i] = v4i{0, 0, 0, 0};
+    const int8_t* a = QUANT ? rows + min(lr, g.M - 1) * ld + 16 * j : g.q + (int64_t)min(m0 + lr, g.M - 1) * g.lda + 16 * j;
+    v4i acc = {0, 0, 0, 0};
     for (int s = from; s < to; s += U) {
         if (s != from) load_b(s);
-        v4i fa[TI][QUANT ? 1 : U];
+        v4i fa[U];
         if constexpr (!QUANT) {
 #pragma unroll
-            for (int i = 0; i < TI; ++i)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    fa[i][u] = *reinterpret_cast<const v4i*>(g.q + (int64_t)min(m0 + 16 * i + lr, g.M - 1) * g.lda + min(s + u, steps - 1) * 64 + 16 * j);
+            for (int u = 0; u < U; ++u) fa[u] = *reinterpret_cast<const v4i*>(a + min(s + u, steps - 1) * 64);
         }
         __builtin_amdgcn_sched_barrier(0);  // every load of the group before the first product
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s + u >= to) break;
-#pragma unroll
-            for (int i = 0; i < TI; ++i) {
-                if constexpr (QUANT) fa[i][0] = *reinterpret_cast<const v4i*>(rows + min(lr, g.M - 1) * ld + (s + u) * 64 + 16 * j);
-                acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i][QUANT ? 0 : u], fb[u], acc[i], 0, 0, 0);
-            }
+            if constexpr (QUANT) fa[u] = *reinterpret_cast<const v4i*>(a + (s + u) * 64);
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u], fb[u], acc, 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int i = 0; i < TI; ++i) part[wid][i][lane] = acc[i];
+    part[wid][lane] = acc;
     __syncthreads();
-    if (wid >= TI) return;
-    v4i sum = part[0][wid][lane];
+    if (wid) return;
 #pragma unroll
-    for (int w = 1; w < W; ++w) sum += part[w][wid][lane];
+    for (int w = 1; w < W; ++w) acc += part[w][lane];
     const int n = n0 + lr;
     if (n >= g.N) return;
     const float ws = g.ws[n], bias = g.bias ? g.bias[n] : 0.0f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int m = m0 + 16 * wid + 4 * j + r;
-        if (m < g.M) reinterpret_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = (T)finish(sum[r], QUANT ? scales[m] : g.xs[m], ws, bias);
+        const int m = m0 + 4 * j + r;
+        if (m < g.M) reinterpret_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = (T)finish(acc[r], QUANT ? scales[m] : g.xs[m], ws, bias);
     }
 }
 
@@ -367,18 +358,17 @@ __device__ __forceinline__ void tile_of(const ProductArgs& g, int& tm, int& tn) 
 
 constexpr int kBig = 256, kStep = 128;
 
-// C channels of one token from n on.
+// C channels of one token from n on, 16 bytes at a time wherever the row starts.
 template <int C, typename T>
-__device__ __forceinline__ void store_channels(T* row, int n, int N, bool wide, const float (&v)[C]) {
+__device__ __forceinline__ void store_channels(T* row, int n, int N, const float (&v)[C]) {
     constexpr int V = 16 / (int)sizeof(T);
-    if (wide && n + C <= N) {
-        typedef T vec __attribute__((ext_vector_type(V)));
+    if (n + C <= N) {
 #pragma unroll
         for (int i = 0; i < C / V; ++i) {
-            vec w;
+            float u[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = (T)v[i * V + e];
-            *reinterpret_cast<vec*>(row + n + i * V) = w;
+            for (int e = 0; e < V; ++e) u[e] = v[i * V + e];
+            icx::store_f32(row + n + i * V, u);
         }
     } else {
 #pragma unroll
@@ -494,7 +484,6 @@ __global__ void __launch_bounds__(512, 2) token_product_big_kernel(ProductArgs g
         ws[e] = g.ws[c];
         bias[e] = g.bias ? g.bias[c] : 0.0f;
     }
-    const bool wide = (g.ldy * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int m = m0 + wm * 128 + i * 16 + lr;
@@ -505,89 +494,111 @@ __global__ void __launch_bounds__(512, 2) token_product_big_kernel(ProductArgs g
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[4 * t + r] = finish(acc[i][t][r], xs, ws[4 * t + r], bias[4 * t + r]);
-        store_channels<16>(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, wide, v);
+        store_channels<16>(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, v);
     }
 }
 
 // ---- between them: tiles of 64 x 64 and 128 x 128 ---------------------------------------------------
-// Four waves, 2 x 2, each half of either side; NS steps of 128 bytes of K stand in LDS, NS - 1 of them on
-// their way, one barrier a step: past it step kt has landed (its copies are waited for by the count of
-// those issued after them) and the buffer that step kt - 1 was read from takes the copies of step
-// kt + NS - 1.  Channels are laid out over a wave's tiles as above, a lane's results 4 TN consecutive ones.
+// WM x WN waves, each its part of a BM x BN tile, and KS such groups of waves, which take the 128-byte steps of
+// K in turn and are added up at the end (integers: the same sum in any order).  A stage is KS steps; NS
+// stages stand in LDS, NS - 1 of them on their way, one barrier a stage: past it stage i has landed (its
+// copies are waited for by the count of those issued after them) and the buffer that stage i - 1 was read
+// from takes the copies of stage i + NS - 1.  Channels are laid out over a wave's tiles as above, a
+// lane's results 4 TN consecutive ones.
+// What bounds small products is the number of stages, some 450 cycles each however little they multiply:
+// two groups of waves halve it (200 x 4096 x 4096: 12.6 -> 10.5 us).
 template <int N>
 __device__ __forceinline__ void wait_copies_but() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
-template <int B, int NS, typename T>
-__global__ void __launch_bounds__(256) token_product_tile_kernel(ProductArgs g) {
-    constexpr int TN = B / 32;  // tiles of 16 on either side of a wave's B / 2
-    constexpr int P = B / 32;   // copies of each operand a wave and step
-    __shared__ __attribute__((aligned(1024))) int8_t smem[NS][2 * B * kStep];
+template <int BM, int BN, int WM, int WN, int KS, int NS, typename T>
+__global__ void __launch_bounds__(64 * WM * WN * KS) token_product_tile_kernel(ProductArgs g) {
+    constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // tiles of 16 of a wave
+    constexpr int P = (BM + BN) / 8 / (WM * WN);         // copies a wave and stage
+    constexpr int PART = (BM + BN) * kStep;
+    static_assert(P * 8 * WM * WN == BM + BN && (TN == 2 || TN == 4), "");
+    static_assert((KS - 1) * TM * TN * 1024 * WM * WN <= NS * KS * PART, "the sums of the other groups fit where the stages were");
+    __shared__ __attribute__((aligned(1024))) int8_t smem[NS][KS][PART];
     int tm, tn;
     tile_of(g, tm, tn);
-    const int m0 = tm * B, n0 = tn * B;
+    const int m0 = tm * BM, n0 = tn * BN;
     const int lane = threadIdx.x & 63, lr = lane & 15, j = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wid >> 1, wn = wid & 1;
+    const int ks = wid / (WM * WN), w = wid % (WM * WN), wm = w / WN, wn = w % WN;
     // bits 1 and the next two of those that tell the 16 rows of a fragment apart
     auto key = [&](int row) { return ((row >> 1) & 1) | ((row / (4 * TN)) & 3) << 1; };
 
+    // this wave's rows of the stage's part ks: tokens, then channels
     const int8_t* qa = g.q + (int64_t)m0 * g.lda;
     const int8_t* wa = g.w + (int64_t)n0 * g.Kp;
-    uint32_t oq[P], ow[P];
+    const int8_t* base[P];
+    uint32_t off[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int row = (wid * P + i) * 8 + (lane >> 3);
-        oq[i] = (uint32_t)((int64_t)min(row, g.M - 1 - m0) * g.lda + 16 * ((lane & 7) ^ token_key(row)));
-        ow[i] = (uint32_t)((int64_t)min(row, g.N - 1 - n0) * g.Kp + 16 * ((lane & 7) ^ key(row)));
+        const int first = (w * P + i) * 8, row = first + (lane >> 3), c = row - BM;
+        base[i] = first < BM ? qa : wa;
+        off[i] = first < BM ? (uint32_t)((int64_t)min(row, g.M - 1 - m0) * g.lda + 16 * ((lane & 7) ^ token_key(row)))
+                            : (uint32_t)((int64_t)min(c, g.N - 1 - n0) * g.Kp + 16 * ((lane & 7) ^ key(c)));
     }
-    const uint32_t lds = lds_address(smem) + wid * P * 8 * kStep;
-    const int KT = g.Kp / kStep;
-    auto copy = [&](int kt) {
-        const uint32_t to = lds + (uint32_t)(kt % NS) * (2 * B * kStep);
-        const int k = min(kt, KT - 1) * kStep;  // past the end: the last step again, into a buffer that nobody reads
+    const uint32_t lds = lds_address(smem) + ks * PART + w * P * 8 * kStep;
+    const int KT = g.Kp / kStep, stages = (KT + KS - 1) / KS;
+    auto copy = [&](int i) {
+        const uint32_t to = lds + (uint32_t)(i % NS) * (KS * PART);
+        const int k = min(i * KS + ks, KT - 1) * kStep;  // past the end: the last step again, which nobody multiplies
 #pragma unroll
-        for (int i = 0; i < P; ++i) copy_to_lds(qa + k, oq[i], to + i * 8 * kStep);
-#pragma unroll
-        for (int i = 0; i < P; ++i) copy_to_lds(wa + k, ow[i], to + B * kStep + i * 8 * kStep);
+        for (int n = 0; n < P; ++n) copy_to_lds(base[n] + k, off[n], to + n * 8 * kStep);
     };
-    v4i acc[TN][TN];
+    v4i acc[TM][TN];
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int t = 0; t < TN; ++t) acc[i][t] = v4i{0, 0, 0, 0};
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) copy(s);
-    for (int kt = 0; kt < KT; ++kt) {
-        wait_copies_but<2 * P * (NS - 2)>();
+    for (int st = 0; st < stages; ++st) {
+        wait_copies_but<P * (NS - 2)>();
         barrier();
-        copy(kt + NS - 1);
-        const int8_t* a = smem[kt % NS];
-        const int8_t* b = a + B * kStep;
+        copy(st + NS - 1);
+        if (KS > 1 && st * KS + ks >= KT) continue;
+        const int8_t* a = smem[st % NS][ks];
+        const int8_t* b = a + BM * kStep;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            v4i fq[TN], fw[TN];
+            v4i fq[TM], fw[TN];
 #pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                const int row = wm * (B / 2) + i * 16 + lr;
+            for (int i = 0; i < TM; ++i) {
+                const int row = wm * (BM / WM) + i * 16 + lr;
                 fq[i] = *reinterpret_cast<const v4i*>(a + row * kStep + 16 * ((4 * k + j) ^ token_key(row)));
             }
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
-                const int row = wn * (B / 2) + (lr >> 2) * 4 * TN + t * 4 + (lr & 3);
+                const int row = wn * (BN / WN) + (lr >> 2) * 4 * TN + t * 4 + (lr & 3);
                 fw[t] = *reinterpret_cast<const v4i*>(b + row * kStep + 16 * ((4 * k + j) ^ key(row)));
             }
 #pragma unroll
-            for (int i = 0; i < TN; ++i)
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int t = 0; t < TN; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fq[i], acc[i][t], 0, 0, 0);
         }
     }
     wait_copies();  // (those past the end)
+    if constexpr (KS > 1) {
+        static_assert(KS == 2, "");
+        __syncthreads();
+        v4i* sums = reinterpret_cast<v4i*>(&smem[0][0][0]) + w * TM * TN * 64 + lane;
+        if (ks) {
+#pragma unroll
+            for (int i = 0; i < TM * TN; ++i) sums[i * 64] = acc[i / TN][i % TN];
+        }
+        __syncthreads();
+        if (ks) return;
+#pragma unroll
+        for (int i = 0; i < TM * TN; ++i) acc[i / TN][i % TN] += sums[i * 64];
+    }
 
     constexpr int C = 4 * TN;  // channels of a lane
-    const int n = n0 + wn * (B / 2) + C * j;
+    const int n = n0 + wn * (BN / WN) + C * j;
     float ws[C], bias[C];
 #pragma unroll
     for (int e = 0; e < C; ++e) {
@@ -595,10 +606,9 @@ __global__ void __launch_bounds__(256) token_product_tile_kernel(ProductArgs g) 
         ws[e] = g.ws[c];
         bias[e] = g.bias ? g.bias[c] : 0.0f;
     }
-    const bool wide = (g.ldy * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int m = m0 + wm * (B / 2) + i * 16 + lr;
+    for (int i = 0; i < TM; ++i) {
+        const int m = m0 + wm * (BM / WM) + i * 16 + lr;
         if (m >= g.M) continue;
         const float xs = g.xs[m];
         float v[C];
@@ -606,7 +616,7 @@ __global__ void __launch_bounds__(256) token_product_tile_kernel(ProductArgs g) 
         for (int t = 0; t < TN; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[4 * t + r] = finish(acc[i][t][r], xs, ws[4 * t + r], bias[4 * t + r]);
-        store_channels<C>(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, wide, v);
+        store_channels<C>(reinterpret_cast<T*>(g.y) + (int64_t)m * g.ldy, n, g.N, v);
     }
 }
 
@@ -631,19 +641,29 @@ int quantize(hipStream_t s, const void* x, int dtype, size_t M, size_t K, int64_
     });
 }
 
-// Which kernel takes an M x N product, and its tile.
+// Which kernel takes a product, and its tile.  With c CUs, and us of a product of 4096 (768) values:
+//  * 16 x 16 tiles with K over 8 waves for a long K and at most c of them: 100 x 512 6.9 against 9.1 with 64 x 64
+//    tiles, 16 x 4096 7.5 / 9.3; past c 64 x 1500 10.5 / 9.1, and of a short K nothing is left to share
+//    out (16 x 4096 4.8 / 4.1);
+//  * 64 x 64 tiles, with two groups of waves while there are at most c (200 x 4096 10.5 against 12.6 with one; past
+//    that 1024 x 1500 19.2 / 15.2, as LDS then holds one block a CU instead of three), to 3 c of them;
+//  * 128 x 128 tiles to 2 c of them: 1024 x 4096 24.2 (8.7) against 30.8 (10.6) with 64 x 64 and 45 (15) with
+//    256 x 256; at 600 x 4096, 640 tiles of 64, 21.8 (8.0) / 22.7 (7.7);
+//  * 256 x 256 tiles: 8192 x 1500 53.8 (20.9) against 68.8 (21.7) with 128 x 128; at 2048 x 4096, 512 tiles of
+//    128, 48.8 (18.1) / 47.2 (15.6).
+enum { kTile16, kTile64Shared, kTile64, kTile128, kTile256 };
 struct Form {
-    int kind;  // 256, 128 or 64 for a tile of that, else 16-token tiles of token_product_small_kernel
-    size_t tile_m, tile_n;
+    int kind;
+    size_t tile;
 };
-Form form_of(size_t M, size_t N) {
-    const size_t cus = (size_t)icx::num_cus();
-    if (M <= 16) return {1, 16, 16};
-    if (M <= 32) return {2, 32, 16};
-    if (M <= 64) return {4, 64, 16};
-    if (icx::cdiv(M, 256) * icx::cdiv(N, 256) * 4 >= 3 * cus) return {256, 256, 256};
-    if (icx::cdiv(M, 128) * icx::cdiv(N, 128) >= cus) return {128, 128, 128};
-    return {64, 64, 64};
+Form form_of(size_t M, size_t K, size_t N) {
+    const size_t c = (size_t)icx::num_cus();
+    const auto tiles = [&](size_t t) { return icx::cdiv(M, t) * icx::cdiv(N, t); };
+    if (K >= 2048 && tiles(16) <= c) return {kTile16, 16};
+    if (tiles(64) <= c) return {kTile64Shared, 64};
+    if (tiles(64) <= 3 * c) return {kTile64, 64};
+    if (tiles(128) <= 2 * c) return {kTile128, 128};
+    return {kTile256, 256};
 }
 // Tokens that every block of the product quantizes for itself, and the LDS that they may take.
 constexpr size_t kFusedTokens = kSmallWaves, kFusedBytes = 128 * 1024;
@@ -737,19 +757,20 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
     g.M = (int)M;
     g.N = (int)N;
     g.Kp = (int)padded(K);
-    const Form form = form_of(M, N);
-    g.tiles_m = (int)icx::cdiv(M, form.tile_m);
-    g.tiles_n = (int)icx::cdiv(N, form.tile_n);
+    const bool few = own && fused(M, K);
+    const Form form = few ? Form{kTile16, 16} : form_of(M, K, N);
+    g.tiles_m = (int)icx::cdiv(M, form.tile);
+    g.tiles_n = (int)icx::cdiv(N, form.tile);
     if ((uint64_t)g.tiles_m * g.tiles_n > 0x7fffff)
         ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu x %zu outputs are too many for a launch", who, M, N);
     const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n);
-    if (own && fused(M, K)) {
+    if (few) {
         const size_t lds = fused_lds(M, K);
         return icx::with_float_type(x_dtype, [&](auto* xt) -> int {
             using X = std::remove_pointer_t<decltype(xt)>;
             return icx::with_float_type(y_dtype, [&](auto* yt) -> int {
                 using T = std::remove_pointer_t<decltype(yt)>;
-                token_product_small_kernel<1, true, X, T><<<blocks, 64 * kSmallWaves, lds, s>>>(g, (const X*)x, x_stride, (int)K);
+                token_product_small_kernel<true, X, T><<<blocks, 64 * kSmallWaves, lds, s>>>(g, (const X*)x, x_stride, (int)K);
                 ICX_LAUNCH_CHECK("token_product_small_kernel");
                 return ICX_OK;
             });
@@ -775,12 +796,11 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
         using T = std::remove_pointer_t<decltype(t)>;
         const int8_t* none = nullptr;
         switch (form.kind) {
-            case 256: token_product_big_kernel<T><<<blocks, 512, 0, s>>>(g); break;
-            case 128: token_product_tile_kernel<128, 2, T><<<blocks, 256, 0, s>>>(g); break;
-            case 64: token_product_tile_kernel<64, 3, T><<<blocks, 256, 0, s>>>(g); break;
-            case 4: token_product_small_kernel<4, false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
-            case 2: token_product_small_kernel<2, false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
-            default: token_product_small_kernel<1, false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
+            case kTile256: token_product_big_kernel<T><<<blocks, 512, 0, s>>>(g); break;
+            case kTile128: token_product_tile_kernel<128, 128, 2, 4, 1, 3, T><<<blocks, 512, 0, s>>>(g); break;
+            case kTile64: token_product_tile_kernel<64, 64, 2, 2, 1, 3, T><<<blocks, 256, 0, s>>>(g); break;
+            case kTile64Shared: token_product_tile_kernel<64, 64, 2, 2, 2, 3, T><<<blocks, 512, 0, s>>>(g); break;
+            default: token_product_small_kernel<false, int8_t, T><<<blocks, 64 * kSmallWaves, 0, s>>>(g, none, 0, 0); break;
         }
         ICX_LAUNCH_CHECK("token_product");
         return ICX_OK;
