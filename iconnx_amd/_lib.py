@@ -45,6 +45,19 @@ class KvCacheDesc(ctypes.Structure):
                 ("kv_heads", ctypes.c_int32), ("head_size", ctypes.c_int32), ("bits", ctypes.c_int32)]
 
 
+class KvWrite(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("k_token_stride", ctypes.c_int64),
+                ("k_head_stride", ctypes.c_int64), ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("tokens", ctypes.c_size_t), ("dtype", ctypes.c_int32), ("slots_dtype", ctypes.c_int32)]
+
+
+class TokenLinear(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("x_scale", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("M", ctypes.c_size_t),
+                ("K", ctypes.c_size_t), ("N", ctypes.c_size_t), ("packed", ctypes.c_void_p), ("w_scale", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("x_dtype", ctypes.c_int32),
+                ("y_dtype", ctypes.c_int32)]
+
+
 class KvAttention(ctypes.Structure):
     _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64),
                 ("q_head_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
@@ -112,9 +125,9 @@ SIGNATURES = {
     "icx_pack_token_weight": ([P, P, S, S, P], I),
     "icx_quantize_tokens": ([P, P, I, S, S, LL, P, P], I),
     "icx_token_qlinear_workspace_size": ([S, S, S, I], S),
-    "icx_token_qlinear": ([P, P, I, LL, P, S, S, S, P, P, P, P, I, LL, P, S], I),
+    "icx_token_qlinear": ([P, P, P, S], I),
     "icx_kv_cache_bytes": ([P], S),
-    "icx_kv_cache_write": ([P, P, P, P, I, S, LL, LL, LL, LL, P, I], I),
+    "icx_kv_cache_write": ([P, P, P], I),
     "icx_kv_cache_read": ([P, P, P, I, S, P, P, I], I),
     "icx_kv_cache_attention_workspace_size": ([P, P], S),
     "icx_kv_cache_attention": ([P, P, P, P, S], I),

@@ -238,23 +238,23 @@ extern "C" size_t icx_kv_cache_bytes(const icx_kv_cache* c) {
     return (size_t)d.pages * (size_t)icx::kv_layout(d).page_bytes;
 }
 
-extern "C" int icx_kv_cache_write(icx_stream_t stream, const icx_kv_cache* cache, const void* k, const void* v, int dtype,
-                                  size_t tokens, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                                  int64_t v_head_stride, const void* slots, int slots_dtype) {
+extern "C" int icx_kv_cache_write(icx_stream_t stream, const icx_kv_cache* cache, const icx_kv_write* args) {
     icx::clear_error();
+    const char* who = "KvCacheWrite";
+    if (!args) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null arguments", who);
     CacheArgs a;
-    int rc = cache_args(cache, slots, slots_dtype, tokens, dtype, "KvCacheWrite", &a);
+    int rc = cache_args(cache, args->slots, args->slots_dtype, args->tokens, args->dtype, who, &a);
     if (rc) return rc;
-    if (tokens == 0) return ICX_OK;
-    if (!k || !v || !slots) ICX_FAIL(ICX_ERR_INVALID_ARG, "KvCacheWrite: null k, v or slots");
-    a.k = k;
-    a.v = v;
-    a.k_token = k_token_stride;
-    a.k_head = k_head_stride;
-    a.v_token = v_token_stride;
-    a.v_head = v_head_stride;
+    if (args->tokens == 0) return ICX_OK;
+    if (!args->k || !args->v || !args->slots) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null k, v or slots", who);
+    a.k = args->k;
+    a.v = args->v;
+    a.k_token = args->k_token_stride;
+    a.k_head = args->k_head_stride;
+    a.v_token = args->v_token_stride;
+    a.v_head = args->v_head_stride;
     const unsigned blocks = (unsigned)icx::cdiv((size_t)a.units * 4, kThreads);
-    return icx::with_float_type(dtype, [&](auto* t) -> int {
+    return icx::with_float_type(args->dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
         if (cache->bits == 4) kv_write_kernel<4, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
         else kv_write_kernel<8, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);

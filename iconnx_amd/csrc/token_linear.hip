@@ -670,12 +670,12 @@ constexpr size_t kFusedTokens = kSmallWaves, kFusedBytes = 128 * 1024;
 inline size_t fused_lds(size_t M, size_t K) { return M * (padded(K) + 16); }
 inline bool fused(size_t M, size_t K) { return M <= kFusedTokens && fused_lds(M, K) <= kFusedBytes; }
 
-// q [M, Kp] and, behind it, the scales (Int8 tokens: room for rows that have to be padded).
+// q [M, Kp] and, behind it, the scales (Int8 tokens: rows that have to be padded).
 struct Workspace {
     size_t scale_off, total;
 };
 Workspace workspace(size_t M, size_t K, int x_dtype) {
-    if (x_dtype != ICX_I8 && fused(M, K)) return {0, 0};
+    if (x_dtype == ICX_I8 ? K % kAlignK == 0 : fused(M, K)) return {0, 0};
     const size_t q = icx::align_up(M * padded(K), 256);
     return {q, q + (x_dtype == ICX_I8 ? 0 : 4 * M)};
 }
@@ -725,35 +725,38 @@ extern "C" size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N,
     return workspace(M, K, x_dtype).total;
 }
 
-extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype, int64_t x_stride, const float* x_scale, size_t M,
-                                 size_t K, size_t N, const int8_t* packed, const float* w_scale, const float* bias, void* y,
-                                 int y_dtype, int64_t y_stride, void* ws, size_t ws_bytes) {
+extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* args, void* ws, size_t ws_bytes) {
     icx::clear_error();
     const char* who = "TokenQLinear";
+    if (!args) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null arguments", who);
+    const icx_token_linear& a = *args;
+    const size_t M = a.M, K = a.K, N = a.N;
     int rc = check_sizes(M, K, N, who);
     if (rc) return rc;
-    const bool own = x_dtype != ICX_I8;
-    if (own && !icx::is_float_kind(x_dtype))
-        ICX_FAIL(ICX_ERR_DTYPE, "%s: x dtype %d unsupported (must be Int8, Float32, Float16 or BFloat16)", who, x_dtype);
-    if (!icx::is_float_kind(y_dtype))
-        ICX_FAIL(ICX_ERR_DTYPE, "%s: y dtype %d unsupported (must be Float32, Float16 or BFloat16)", who, y_dtype);
-    if (own == (x_scale != nullptr))
-        ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: Int8 tokens come with their scales, others without (x dtype %d, scales %s)", who, x_dtype,
-                 x_scale ? "given" : "missing");
+    const bool own = a.x_dtype != ICX_I8;
+    if (own && !icx::is_float_kind(a.x_dtype))
+        ICX_FAIL(ICX_ERR_DTYPE, "%s: x dtype %d unsupported (must be Int8, Float32, Float16 or BFloat16)", who, a.x_dtype);
+    if (!icx::is_float_kind(a.y_dtype))
+        ICX_FAIL(ICX_ERR_DTYPE, "%s: y dtype %d unsupported (must be Float32, Float16 or BFloat16)", who, a.y_dtype);
+    if (own == (a.x_scale != nullptr))
+        ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: Int8 tokens come with their scales, others without (x dtype %d, scales %s)", who,
+                 a.x_dtype, a.x_scale ? "given" : "missing");
     if (M == 0 || N == 0) return ICX_OK;
-    if (!x || !packed || !w_scale || !y) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null x, weight, scale or y", who);
-    if (!icx::aligned16(packed)) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: the packed weight must be 16-byte aligned", who);
-    const Workspace L = workspace(M, K, x_dtype);
-    const bool pad = !own && (K % kAlignK || x_stride % 16 || !icx::aligned16(x));
-    if ((own || pad) && L.total && (!ws || ws_bytes < L.total))
+    if (!a.x || !a.packed || !a.w_scale || !a.y) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null x, weight, scale or y", who);
+    if (!icx::aligned16(a.packed)) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: the packed weight must be 16-byte aligned", who);
+    const bool pad = !own && K % kAlignK;
+    if (!own && !pad && (a.x_stride % 16 || !icx::aligned16(a.x)))
+        ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: Int8 rows of whole 128 bytes must stand at multiples of 16", who);
+    const Workspace L = workspace(M, K, a.x_dtype);
+    if (L.total && (!ws || ws_bytes < L.total))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, L.total, ws_bytes);
     const hipStream_t s = (hipStream_t)stream;
     ProductArgs g{};
-    g.w = packed;
-    g.ws = w_scale;
-    g.bias = bias;
-    g.y = y;
-    g.ldy = y_stride;
+    g.w = a.packed;
+    g.ws = a.w_scale;
+    g.bias = a.bias;
+    g.y = a.y;
+    g.ldy = a.y_stride;
     g.M = (int)M;
     g.N = (int)N;
     g.Kp = (int)padded(K);
@@ -766,33 +769,33 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype
     const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n);
     if (few) {
         const size_t lds = fused_lds(M, K);
-        return icx::with_float_type(x_dtype, [&](auto* xt) -> int {
+        return icx::with_float_type(a.x_dtype, [&](auto* xt) -> int {
             using X = std::remove_pointer_t<decltype(xt)>;
-            return icx::with_float_type(y_dtype, [&](auto* yt) -> int {
+            return icx::with_float_type(a.y_dtype, [&](auto* yt) -> int {
                 using T = std::remove_pointer_t<decltype(yt)>;
-                token_product_small_kernel<true, X, T><<<blocks, 64 * kSmallWaves, lds, s>>>(g, (const X*)x, x_stride, (int)K);
+                token_product_small_kernel<true, X, T><<<blocks, 64 * kSmallWaves, lds, s>>>(g, (const X*)a.x, a.x_stride, (int)K);
                 ICX_LAUNCH_CHECK("token_product_small_kernel");
                 return ICX_OK;
             });
         });
     }
-    g.q = (const int8_t*)x;
-    g.lda = x_stride;
-    g.xs = x_scale;
+    g.q = (const int8_t*)a.x;
+    g.lda = a.x_stride;
+    g.xs = a.x_scale;
     if (own) {
         float* sc = reinterpret_cast<float*>((char*)ws + L.scale_off);
-        rc = quantize(s, x, x_dtype, M, K, x_stride, (int8_t*)ws, padded(K), padded(K), sc);
+        rc = quantize(s, a.x, a.x_dtype, M, K, a.x_stride, (int8_t*)ws, padded(K), padded(K), sc);
         if (rc) return rc;
         g.q = (const int8_t*)ws;
         g.lda = (int64_t)padded(K);
         g.xs = sc;
     } else if (pad) {
-        token_pad_kernel<<<(unsigned)M, kThreads, 0, s>>>((const int8_t*)x, x_stride, (int)K, (int)padded(K), (int8_t*)ws);
+        token_pad_kernel<<<(unsigned)M, kThreads, 0, s>>>((const int8_t*)a.x, a.x_stride, (int)K, (int)padded(K), (int8_t*)ws);
         ICX_LAUNCH_CHECK("token_pad_kernel");
         g.q = (const int8_t*)ws;
         g.lda = (int64_t)padded(K);
     }
-    return icx::with_float_type(y_dtype, [&](auto* t) -> int {
+    return icx::with_float_type(a.y_dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
         const int8_t* none = nullptr;
         switch (form.kind) {

@@ -29,7 +29,7 @@ import torch
 
 from ._lib import (BCAST_COL, BCAST_FULL, BCAST_ROW, BCAST_SCALAR, ICX_BF16, ICX_F16, ICX_F32, ICX_I8, ICX_I32,
                    ICX_I64, ICX_U8, MAX_CHAIN, OP_ADD, OP_DIV, OP_ERF, OP_MUL, OP_MUL_SAVED, OP_SAVE,
-                   OP_SUB, Chain, IconnxError, KvAttention, KvCacheDesc, check, lib)
+                   OP_SUB, Chain, IconnxError, KvAttention, KvCacheDesc, KvWrite, TokenLinear, check, lib)
 
 ERR_SHAPE, ERR_DTYPE, ERR_INVALID, ERR_UNSUPPORTED = 2, 3, 1, 6
 _DT = {torch.int8: ICX_I8, torch.uint8: ICX_U8, torch.int32: ICX_I32, torch.float32: ICX_F32}
@@ -654,10 +654,16 @@ def gpu_quantize_tokens(x):
     _on_device(who, _here(), x)
     M, ld, x = _rows(x)
     dev = x.device
+    shape = tuple(shape)  # (as a tuple: torch.empty takes a Size half as fast)
     q = _empty(shape, dtype=_I8, device=dev)
     scale = _empty(shape[:-1], dtype=_F32, device=dev)
     check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, shape[-1], ld, q.data_ptr(), scale.data_ptr()))
     return q, scale
+
+
+# (arguments by struct: packing thirteen values costs a fifth of converting them one by one)
+_LINEAR_PACK = struct.Struct("=QQqQQQQQQQqii")
+assert _LINEAR_PACK.size == ctypes.sizeof(TokenLinear)
 
 
 def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
@@ -691,25 +697,27 @@ def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
             raise IconnxError(ERR_SHAPE, "%s: bias must be Float32 [%d], got %s %s" % (who, N, _name(bias.dtype), list(bias.shape)))
         _on_device(who, here, bias)
         bias = _dense(bias)
-    oshape = shape[:-1] + (N,)
+    oshape = tuple(shape)[:-1] + (N,)
     if out is not None:
         if out.dtype != yt or out.shape != oshape or not out.is_contiguous():
             raise IconnxError(ERR_SHAPE, "%s: out must be a contiguous %s %s" % (who, _name(yt), list(oshape)))
         _on_device(who, here, out)
     M, ld, x = _rows(x)
+    if code == ICX_I8 and K % 128 == 0 and (ld | x.data_ptr()) % 16:  # rows that the products cannot read in place
+        ld, x = K, x.clone(memory_format=torch.contiguous_format)
     L = lib()
     nws = w._ws.get((M, code))
     if nws is None:
         if len(w._ws) > 4096:  # (a size for each number of tokens that came by)
             w._ws.clear()
         nws = w._ws[(M, code)] = L.icx_token_qlinear_workspace_size(M, K, N, code)
-    dev = x.device
-    y = _empty(oshape, dtype=yt, device=dev) if out is None else out
-    ws = _empty(nws, dtype=_U8, device=dev) if nws else None
-    check(L.icx_token_qlinear(_stream(), x.data_ptr(), code, ld, None if x_scale is None else x_scale.data_ptr(), M, K, N,
-                              w.packed.data_ptr(), w.scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
-                              ycode, N, None if ws is None else ws.data_ptr(), nws))
-    return y
+    if out is None:
+        out = x.new_empty(oshape) if yt == x.dtype else _empty(oshape, dtype=yt, device=x.device)
+    ws = _empty(nws, dtype=_U8, device=x.device) if nws else None
+    args = _LINEAR_PACK.pack(x.data_ptr(), 0 if x_scale is None else x_scale.data_ptr(), ld, M, K, N, w.packed.data_ptr(),
+                             w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), N, code, ycode)
+    check(L.icx_token_qlinear(_stream(), args, None if ws is None else ws.data_ptr(), nws))
+    return out
 
 
 class KvCache:
@@ -740,6 +748,10 @@ def _check_slots(slots, who):
     return code
 
 
+_WRITE_PACK = struct.Struct("=QQQqqqqQii")
+assert _WRITE_PACK.size == ctypes.sizeof(KvWrite)
+
+
 def gpu_kv_cache_write(cache, k, v, slots):
     """Quantizes k and v [tokens, kv_heads, head_size] (any strides with dense heads) into the cache's
     ``slots`` [tokens]; a slot outside the cache, as -1, is passed over."""
@@ -763,7 +775,8 @@ def gpu_kv_cache_write(cache, k, v, slots):
     if one != 1:
         v = v.contiguous()
         vt, vh, _ = v.stride()
-    check(lib().icx_kv_cache_write(_stream(), cache, k.data_ptr(), v.data_ptr(), code, n, kt, kh, vt, vh, slots.data_ptr(), sc))
+    check(lib().icx_kv_cache_write(_stream(), cache, _WRITE_PACK.pack(k.data_ptr(), v.data_ptr(), slots.data_ptr(), kt, kh, vt, vh, n,
+                                                                     code, sc)))
 
 
 def gpu_kv_cache_read(cache, slots, dtype=torch.float32):
@@ -831,7 +844,7 @@ def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_row
         q_starts = _dense(q_starts)
     dev = q.device
     if out is None:
-        out = _empty(shape, dtype=q.dtype, device=dev)
+        out = q.new_empty((rows, heads, D))
     orow, oh, _ = out.stride()
     if max_rows is None:
         max_rows = 1 if q_starts is None else rows

@@ -346,13 +346,24 @@ int icx_pack_token_weight(icx_stream_t stream, const int8_t* b, size_t K, size_t
 /* q [M, K] dense and scale [M] of x [M, K] (row stride x_stride). */
 int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dtype, size_t M, size_t K, int64_t x_stride, int8_t* q,
                         float* scale);
-/* x: ICX_I8 with x_scale [M] (icx_quantize_tokens' outputs, for several products over one input), or a
- * float type with x_scale NULL, quantized on the way.  y [M, N] of y_dtype, row stride y_stride;
- * bias [N] f32 or NULL.  Few tokens need no workspace (0). */
+/* x [M, K]: ICX_I8 with x_scale [M] (icx_quantize_tokens' outputs, for several products over one input),
+ * or a float type with x_scale NULL, quantized on the way.  Int8 rows of whole 128 bytes (K % 128 == 0)
+ * are read in place and have to stand at multiples of 16 bytes (ICX_ERR_INVALID_ARG).  y [M, N]; bias [N]
+ * f32 or NULL.  The workspace may be 0. */
+typedef struct icx_token_linear {
+    const void* x;
+    const float* x_scale;
+    int64_t x_stride;
+    size_t M, K, N;
+    const int8_t* packed;
+    const float* w_scale;
+    const float* bias;
+    void* y;
+    int64_t y_stride;
+    int32_t x_dtype, y_dtype;
+} icx_token_linear;
 size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N, int x_dtype);
-int icx_token_qlinear(icx_stream_t stream, const void* x, int x_dtype, int64_t x_stride, const float* x_scale, size_t M,
-                      size_t K, size_t N, const int8_t* packed, const float* w_scale, const float* bias, void* y, int y_dtype,
-                      int64_t y_stride, void* workspace, size_t workspace_bytes);
+int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* args, void* workspace, size_t workspace_bytes);
 
 /* A paged cache of keys and values in 4 or 8 bits.  A head of head_size values (a multiple of 32 up to
  * 256) is cut into blocks of 32 with a power-of-two scale 2^e each; 4 bits hold the magnitudes 0, 0.5,
@@ -370,9 +381,16 @@ size_t icx_kv_cache_bytes(const icx_kv_cache* cache); /* 0 for a cache that is n
 /* Quantizes k, v [tokens, kv_heads, head_size] (token and head strides given) into the slots
  * (page * page_size + place in it; ICX_I32 or ICX_I64, on the device).  A slot outside the cache, as a
  * negative one, is passed over.  A slot named twice in one call keeps codes of either token. */
-int icx_kv_cache_write(icx_stream_t stream, const icx_kv_cache* cache, const void* k, const void* v, int dtype, size_t tokens,
-                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
-                       const void* slots, int slots_dtype);
+typedef struct icx_kv_write {
+    const void* k;
+    const void* v;
+    const void* slots;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    size_t tokens;
+    int32_t dtype; /* of k and v */
+    int32_t slots_dtype;
+} icx_kv_write;
+int icx_kv_cache_write(icx_stream_t stream, const icx_kv_cache* cache, const icx_kv_write* args);
 /* Reads the slots back into k, v [tokens, kv_heads, head_size] (either may be NULL); zeros for a slot
  * outside the cache. */
 int icx_kv_cache_read(icx_stream_t stream, const icx_kv_cache* cache, const void* slots, int slots_dtype, size_t tokens, void* k,

@@ -28,7 +28,7 @@ def test_caches_that_are_refused(L, kw, status):
     c = ctypes.byref(cache(**kw))
     if kw.get("data", PTR) == PTR:
         assert L.icx_kv_cache_bytes(c) == 0
-    assert L.icx_kv_cache_write(None, c, PTR, PTR, F32, 1, 128, 64, 128, 64, PTR, I32) == status
+    assert L.icx_kv_cache_write(None, c, ctypes.byref(_lib.KvWrite(PTR, PTR, PTR, 128, 64, 128, 64, 1, F32, I32))) == status
     assert L.icx_last_error()
     assert L.icx_kv_cache_read(None, c, PTR, I32, 1, PTR, PTR, F32) == status
     assert L.icx_kv_cache_attention(None, c, ctypes.byref(attention()), None, 0) == status
@@ -70,8 +70,9 @@ def test_cache_writes_and_reads_that_are_refused(L):
     c = ctypes.byref(cache())
 
     def write(k=PTR, v=PTR, dtype=F32, tokens=1, slots=PTR, st=I64):
-        return L.icx_kv_cache_write(None, c, k, v, dtype, tokens, 128, 64, 128, 64, slots, st)
+        return L.icx_kv_cache_write(None, c, ctypes.byref(_lib.KvWrite(k, v, slots, 128, 64, 128, 64, tokens, dtype, st)))
 
+    assert L.icx_kv_cache_write(None, c, None) == BAD
     assert write(dtype=I8) == DTYPE and write(st=F32) == DTYPE
     assert write(k=None) == BAD and write(v=None) == BAD and write(slots=None) == BAD
     assert write(tokens=1 << 40) == UNSUPPORTED and write(tokens=(1 << 64) - 1) == SHAPE
@@ -82,8 +83,13 @@ def test_cache_writes_and_reads_that_are_refused(L):
 
 
 def test_products_that_are_refused(L):
-    def run(x=PTR, xt=BF16, xs=None, M=2, K=64, N=32, w=PTR, ws=PTR, y=PTR, yt=F32, work=None, n=0):
-        return L.icx_token_qlinear(None, x, xt, K, xs, M, K, N, w, ws, None, y, yt, N, work, n)
+    def run(x=PTR, xt=BF16, xs=None, M=2, K=64, N=32, w=PTR, ws=PTR, y=PTR, yt=F32, work=None, n=0, ld=None):
+        args = _lib.TokenLinear(x, xs, K if ld is None else ld, M, K, N, w, ws, None, y, N, xt, yt)
+        return L.icx_token_qlinear(None, ctypes.byref(args), work, n)
+
+    assert L.icx_token_qlinear(None, None, None, 0) == BAD
+    assert run(xt=I8, xs=PTR, K=128, x=PTR + 1) == BAD and run(xt=I8, xs=PTR, K=128, ld=130) == BAD
+    assert run(xt=I8, xs=PTR, K=100) == WORKSPACE  # (rows that have to be padded)
 
     assert run(xt=I32) == DTYPE and run(yt=I8) == DTYPE
     assert run(xs=PTR) == BAD and run(xt=I8) == BAD
