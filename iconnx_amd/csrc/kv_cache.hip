@@ -3,8 +3,13 @@
 //
 // Four lanes share a block of 32 values.  A lane takes 8 consecutive keys (its codes are then a
 // whole dword or two of the token's row), and of the values 4 consecutive ones of each half of the
-// block, the pairs that a byte of the transposed layout holds.  Both kernels are bound by memory;
-// the conversions are one instruction a pair.
+// block, the pairs that a byte of the transposed layout holds.  The conversions are one instruction a
+// pair; what bounds the kernels is memory, and how it is reached.  A token alone leaves its values' codes
+// in bytes apart, each an access of its own; so for many tokens a wave takes 16 of them and one head, and
+// where their slots are a chunk of 16 from its start on, as a prompt's are, the chunk goes through LDS and to
+// memory in whole lines (kv_write_chunks_kernel, kv_read_chunks_kernel).
+#include <type_traits>
+
 #include "kv_format.hpp"
 
 namespace {
@@ -77,6 +82,24 @@ __device__ __forceinline__ uint2 encode8(float (&v)[8], uint32_t eb) {
     }
 }
 
+// A lane's codes, and the block's scales from its first lane, into a chunk.
+template <int BITS>
+__device__ __forceinline__ void put_codes(uint8_t* c, int G, int t16, int g, int i, uint2 kc, uint2 vc, uint32_t ke, uint32_t ve) {
+    uint8_t* kd = c + (t16 * G + g) * 4 * BITS + i * BITS;
+    if (BITS == 4) *reinterpret_cast<uint32_t*>(kd) = kc.x;
+    else *reinterpret_cast<uint2*>(kd) = kc;
+    uint8_t* vd = c + icx::kv_codes(G, BITS) + (((t16 >> 2) * 16 + 4 * i) * G + g) * BITS + (t16 & 3) * (BITS / 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (BITS == 4) vd[e * G * BITS] = (uint8_t)(vc.x >> (8 * e));
+        else *reinterpret_cast<uint16_t*>(vd + e * G * BITS) = (uint16_t)((e < 2 ? vc.x : vc.y) >> (16 * (e & 1)));
+    }
+    if (i == 0) {
+        c[icx::kv_key_scales(G, BITS) + t16 * G + g] = (uint8_t)ke;
+        c[icx::kv_value_scales(G, BITS) + ((t16 >> 2) * G + g) * 4 + (t16 & 3)] = (uint8_t)ve;
+    }
+}
+
 template <int BITS, typename T>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(CacheArgs a) {
     const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -109,25 +132,58 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(CacheArgs a) {
     const uint2 kc = encode8<BITS>(k, ke), vc = encode8<BITS>(v, ve);
     int t16;
     uint8_t* c = chunk_of(a, slot, h, t16);
-    const int codes = icx::kv_codes(G, BITS);
-    uint8_t* kd = c + (t16 * G + g) * 4 * BITS + i * BITS;
-    if (BITS == 4) *reinterpret_cast<uint32_t*>(kd) = kc.x;
-    else *reinterpret_cast<uint2*>(kd) = kc;
-    uint8_t* vd = c + codes + (((t16 >> 2) * 16 + 4 * i) * G + g) * BITS + (t16 & 3) * (BITS / 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (BITS == 4) vd[e * G * BITS] = (uint8_t)(vc.x >> (8 * e));
-        else *reinterpret_cast<uint16_t*>(vd + e * G * BITS) = (uint16_t)((e < 2 ? vc.x : vc.y) >> (16 * (e & 1)));
-    }
-    if (i == 0) {
-        c[icx::kv_key_scales(G, BITS) + t16 * G + g] = (uint8_t)ke;
-        c[icx::kv_value_scales(G, BITS) + ((t16 >> 2) * G + g) * 4 + (t16 & 3)] = (uint8_t)ve;
-    }
+    put_codes<BITS>(c, G, t16, g, i, kc, vc, ke, ve);
 }
 
 __device__ __forceinline__ void unpack(uint32_t w, float& lo, float& hi) {
     lo = __uint_as_float(w << 16);
     hi = __uint_as_float(w & 0xffff0000u);
+}
+
+// A lane's values from a chunk, and into the outputs.
+template <int BITS>
+__device__ __forceinline__ void take_codes(const uint8_t* c, int G, int t16, int g, int i, float (&k)[8], float (&v)[8]) {
+    const int codes = icx::kv_codes(G, BITS);
+    const uint8_t* kd = c + (t16 * G + g) * 4 * BITS + i * BITS;
+    const uint8_t* vd = c + codes + (((t16 >> 2) * 16 + 4 * i) * G + g) * BITS + (t16 & 3) * (BITS / 4);
+    const float ks = icx::scale_of(c[icx::kv_key_scales(G, BITS) + t16 * G + g], 0);
+    const float vs = icx::scale_of(c[icx::kv_value_scales(G, BITS) + ((t16 >> 2) * G + g) * 4 + (t16 & 3)], 0);
+    if constexpr (BITS == 4) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(kd);
+        unpack(icx::decode2<4, 0>(w, ks), k[0], k[1]);
+        unpack(icx::decode2<4, 1>(w, ks), k[2], k[3]);
+        unpack(icx::decode2<4, 2>(w, ks), k[4], k[5]);
+        unpack(icx::decode2<4, 3>(w, ks), k[6], k[7]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) unpack(icx::decode2<4, 0>(vd[e * G * BITS], vs), v[e], v[4 + e]);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(kd);
+        unpack(icx::decode2<8, 0>(w.x, ks), k[0], k[1]);
+        unpack(icx::decode2<8, 1>(w.x, ks), k[2], k[3]);
+        unpack(icx::decode2<8, 0>(w.y, ks), k[4], k[5]);
+        unpack(icx::decode2<8, 1>(w.y, ks), k[6], k[7]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            unpack(icx::decode2<8, 0>(*reinterpret_cast<const uint16_t*>(vd + e * G * BITS), vs), v[e], v[4 + e]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_values(const CacheArgs& a, int64_t t, int h, int G, int g, int i, const float (&k)[8],
+                                           const float (&v)[8]) {
+    const int64_t row = (t * a.l.heads + h) * (32 * (int64_t)G) + 32 * g;
+    if (a.k_out) icx::store_f32(reinterpret_cast<T*>(a.k_out) + row + 8 * i, k);
+    if (a.v_out) {
+        float lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            lo[e] = v[e];
+            hi[e] = v[4 + e];
+        }
+        T* vo = reinterpret_cast<T*>(a.v_out) + row + 4 * i;
+        icx::store_f32(vo, lo);
+        icx::store_f32(vo + 16, hi);
+    }
 }
 
 template <int BITS, typename T>
@@ -149,42 +205,133 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(CacheArgs a) {
     } else {
         int t16;
         const uint8_t* c = chunk_of(a, slot, h, t16);
-        const int codes = icx::kv_codes(G, BITS);
-        const uint8_t* kd = c + (t16 * G + g) * 4 * BITS + i * BITS;
-        const uint8_t* vd = c + codes + (((t16 >> 2) * 16 + 4 * i) * G + g) * BITS + (t16 & 3) * (BITS / 4);
-        const float ks = icx::scale_of(c[icx::kv_key_scales(G, BITS) + t16 * G + g], 0);
-        const float vs = icx::scale_of(c[icx::kv_value_scales(G, BITS) + ((t16 >> 2) * G + g) * 4 + (t16 & 3)], 0);
-        if constexpr (BITS == 4) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(kd);
-            unpack(icx::decode2<4, 0>(w, ks), k[0], k[1]);
-            unpack(icx::decode2<4, 1>(w, ks), k[2], k[3]);
-            unpack(icx::decode2<4, 2>(w, ks), k[4], k[5]);
-            unpack(icx::decode2<4, 3>(w, ks), k[6], k[7]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) unpack(icx::decode2<4, 0>(vd[e * G * BITS], vs), v[e], v[4 + e]);
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(kd);
-            unpack(icx::decode2<8, 0>(w.x, ks), k[0], k[1]);
-            unpack(icx::decode2<8, 1>(w.x, ks), k[2], k[3]);
-            unpack(icx::decode2<8, 0>(w.y, ks), k[4], k[5]);
-            unpack(icx::decode2<8, 1>(w.y, ks), k[6], k[7]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                unpack(icx::decode2<8, 0>(*reinterpret_cast<const uint16_t*>(vd + e * G * BITS), vs), v[e], v[4 + e]);
-        }
+        take_codes<BITS>(c, G, t16, g, i, k, v);
     }
-    const int64_t row = (t * a.l.heads + h) * (32 * (int64_t)G) + 32 * g;
-    if (a.k_out) icx::store_f32(reinterpret_cast<T*>(a.k_out) + row + 8 * i, k);
-    if (a.v_out) {
+    put_values<T>(a, t, h, G, g, i, k, v);
+}
+
+// ---- 16 tokens and one head a wave ----------------------------------------------------------------
+// The tokens 16 n - d .. + 15, d the place of the first slot in its chunk: a prompt that starts inside a chunk
+// still meets the chunks after it from their start.
+struct Sixteen {
+    int64_t first;  // of the list; some may lie outside it
+    int head;
+    bool chunk;     // the slots are one chunk
+    uint8_t* at;    // of that chunk
+};
+
+template <int W>
+__device__ __forceinline__ Sixteen sixteen(const CacheArgs& a, int64_t (&slots)[W][16], int wid, int lane) {
+    Sixteen s;
+    const int64_t n = (int64_t)blockIdx.x * W + wid;
+    s.head = (int)(n % a.l.heads);
+    s.first = n / a.l.heads * 16 - (slot_of(a, 0) & 15);
+    int64_t slot = -1;
+    const int64_t t = s.first + (lane & 15);
+    if (t >= 0 && t < a.tokens) slot = slot_of(a, t);
+    if (slot >= a.slots_end) slot = -1;
+    if (lane < 16) slots[wid][lane] = slot;
+    const int lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)slot), hi = __builtin_amdgcn_readfirstlane((int)(slot >> 32));
+    const int64_t base = (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+    s.chunk = __all(base >= 0 && (base & 15) == 0 && slot == base + (lane & 15));
+    int t16;
+    s.at = chunk_of(a, s.chunk ? base : 0, s.head, t16);
+    __syncthreads();
+    return s;
+}
+
+// Piece p of the wave's 64 G: block g of token t, lane i of its four.
+template <int G>
+__device__ __forceinline__ void piece(int p, int& t, int& g, int& i) {
+    t = p / (4 * G);
+    g = p % (4 * G) >> 2;
+    i = p & 3;
+}
+
+template <int BITS, int G, typename T>
+__global__ void __launch_bounds__(kThreads) kv_write_chunks_kernel(CacheArgs a) {
+    constexpr int W = kThreads / 64, BYTES = 2 * (64 * G * BITS + 16 * G);
+    __shared__ __attribute__((aligned(16))) uint8_t image[W][BYTES];
+    __shared__ int64_t slots[W][16];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Sixteen s = sixteen<W>(a, slots, wid, lane);
+    float k[G][8], v[G][8];
+#pragma unroll
+    for (int n = 0; n < G; ++n) {
+        int t, g, i;
+        piece<G>(n * 64 + lane, t, g, i);
+        const int64_t tok = min(max(s.first + t, (int64_t)0), a.tokens - 1);
+        icx::load_f32(reinterpret_cast<const T*>(a.k) + tok * a.k_token + s.head * a.k_head + 32 * g + 8 * i, k[n]);
+        const T* vp = reinterpret_cast<const T*>(a.v) + tok * a.v_token + s.head * a.v_head + 32 * g + 4 * i;
         float lo[4], hi[4];
+        icx::load_f32(vp, lo);
+        icx::load_f32(vp + 16, hi);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            lo[e] = v[e];
-            hi[e] = v[4 + e];
+            v[n][2 * e] = lo[e];
+            v[n][2 * e + 1] = hi[e];
         }
-        T* vo = reinterpret_cast<T*>(a.v_out) + row + 4 * i;
-        icx::store_f32(vo, lo);
-        icx::store_f32(vo + 16, hi);
+    }
+#pragma unroll
+    for (int n = 0; n < G; ++n) {
+        int t, g, i;
+        piece<G>(n * 64 + lane, t, g, i);
+        const uint32_t ke = icx::block_exponent<BITS>(block_top(k[n])), ve = icx::block_exponent<BITS>(block_top(v[n]));
+        const uint2 kc = encode8<BITS>(k[n], ke), vc = encode8<BITS>(v[n], ve);
+        uint8_t* c = image[wid];
+        int t16 = t;
+        if (!s.chunk) {
+            const int64_t slot = slots[wid][t];
+            if (slot < 0) continue;
+            c = chunk_of(a, slot, s.head, t16);
+        }
+        put_codes<BITS>(c, G, t16, g, i, kc, vc, ke, ve);
+    }
+    __syncthreads();
+    if (!s.chunk) return;
+    const uint4* from = reinterpret_cast<const uint4*>(image[wid]);
+    uint4* to = reinterpret_cast<uint4*>(s.at);
+#pragma unroll
+    for (int n = 0; n < (BYTES / 16 + 63) / 64; ++n)
+        if (n * 64 + lane < BYTES / 16) to[n * 64 + lane] = from[n * 64 + lane];
+}
+
+template <int BITS, int G, typename T>
+__global__ void __launch_bounds__(kThreads) kv_read_chunks_kernel(CacheArgs a) {
+    constexpr int W = kThreads / 64, BYTES = 2 * (64 * G * BITS + 16 * G);
+    __shared__ __attribute__((aligned(16))) uint8_t image[W][BYTES];
+    __shared__ int64_t slots[W][16];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Sixteen s = sixteen<W>(a, slots, wid, lane);
+    if (s.chunk) {
+        const uint4* from = reinterpret_cast<const uint4*>(s.at);
+        uint4* to = reinterpret_cast<uint4*>(image[wid]);
+#pragma unroll
+        for (int n = 0; n < (BYTES / 16 + 63) / 64; ++n)
+            if (n * 64 + lane < BYTES / 16) to[n * 64 + lane] = from[n * 64 + lane];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < G; ++n) {
+        int t, g, i;
+        piece<G>(n * 64 + lane, t, g, i);
+        const int64_t tok = s.first + t;
+        if (tok < 0 || tok >= a.tokens) continue;
+        float k[8], v[8];
+        if (s.chunk) {
+            take_codes<BITS>(image[wid], G, t, g, i, k, v);
+        } else {
+            const int64_t slot = slots[wid][t];
+            if (slot >= 0) {
+                int t16;
+                const uint8_t* c = chunk_of(a, slot, s.head, t16);
+                take_codes<BITS>(c, G, t16, g, i, k, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.0f;
+            }
+        }
+        put_values<T>(a, tok, s.head, G, g, i, k, v);
     }
 }
 
@@ -211,6 +358,36 @@ int cache_args(const icx_kv_cache* c, const void* slots, int slots_dtype, size_t
     // HIP's limit on the threads of a launch is 2^32 - 1
     if (a->units > (int64_t)0x3fffffff) ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu tokens a call are too many", who, tokens);
     return ICX_OK;
+}
+
+// From how many heads of tokens on the kernels of 16 tokens a wave are taken.  8 heads of 128, 4 bits, us of
+// either kernel: writes of 1024 tokens 3.9 / 4.4, of 2048 5.3 / 4.5, of 16384 19.7 / 13.3 (slots out of
+// order 3.9 / 5.6, 5.4 / 6.1, 20.5 / 20.9); reads of 4096 6.3 / 6.8, of 16384 18.1 / 16.2, and of heads of
+// 256 in float32 17.3 / 15.6 and 72.7 / 48.2.  12289 tokens of 12 heads of 64, 8 bits: written in 20.7 / 12.1,
+// read in 15.2 / 11.6; 65536 of 8 heads of 128 read in 93 / 75 (5.4 TB/s).
+constexpr int64_t kWriteByChunks = 16384, kReadByChunks = 32768;
+unsigned chunk_blocks(const CacheArgs& a) {
+    // (a group more for the tokens before the first whole one)
+    return (unsigned)icx::cdiv((icx::cdiv((size_t)a.tokens, 16) + 1) * (size_t)a.l.heads, kThreads / 64);
+}
+template <int BITS, typename F>
+void with_head(int G, F f) {
+    std::integral_constant<int, BITS> bits;
+    switch (G) {
+        case 1: f(bits, std::integral_constant<int, 1>()); break;
+        case 2: f(bits, std::integral_constant<int, 2>()); break;
+        case 3: f(bits, std::integral_constant<int, 3>()); break;
+        case 4: f(bits, std::integral_constant<int, 4>()); break;
+        case 5: f(bits, std::integral_constant<int, 5>()); break;
+        case 6: f(bits, std::integral_constant<int, 6>()); break;
+        case 7: f(bits, std::integral_constant<int, 7>()); break;
+        default: f(bits, std::integral_constant<int, 8>()); break;
+    }
+}
+template <typename F>
+void with_blocks(const icx::KvLayout& l, F f) {
+    if (l.bits == 4) with_head<4>(l.G, f);
+    else with_head<8>(l.G, f);
 }
 
 }  // namespace
@@ -256,7 +433,12 @@ extern "C" int icx_kv_cache_write(icx_stream_t stream, const icx_kv_cache* cache
     const unsigned blocks = (unsigned)icx::cdiv((size_t)a.units * 4, kThreads);
     return icx::with_float_type(args->dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (cache->bits == 4) kv_write_kernel<4, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
+        if (a.tokens * a.l.heads >= kWriteByChunks) 
+            with_blocks(a.l, [&](auto bits, auto g) {
+                constexpr int B = decltype(bits)::value, G = decltype(g)::value;
+                kv_write_chunks_kernel<B, G, T><<<chunk_blocks(a), kThreads, 0, (hipStream_t)stream>>>(a);
+            });
+        else if (cache->bits == 4) kv_write_kernel<4, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
         else kv_write_kernel<8, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
         ICX_LAUNCH_CHECK("kv_write_kernel");
         return ICX_OK;
@@ -276,7 +458,12 @@ extern "C" int icx_kv_cache_read(icx_stream_t stream, const icx_kv_cache* cache,
     const unsigned blocks = (unsigned)icx::cdiv((size_t)a.units * 4, kThreads);
     return icx::with_float_type(dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (cache->bits == 4) kv_read_kernel<4, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
+        if (a.tokens * a.l.heads >= kReadByChunks) 
+            with_blocks(a.l, [&](auto bits, auto g) {
+                constexpr int B = decltype(bits)::value, G = decltype(g)::value;
+                kv_read_chunks_kernel<B, G, T><<<chunk_blocks(a), kThreads, 0, (hipStream_t)stream>>>(a);
+            });
+        else if (cache->bits == 4) kv_read_kernel<4, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
         else kv_read_kernel<8, T><<<blocks, kThreads, 0, (hipStream_t)stream>>>(a);
         ICX_LAUNCH_CHECK("kv_read_kernel");
         return ICX_OK;

@@ -63,6 +63,38 @@ def test_runs_of_consecutive_slots(T, first, bits, dtype):
     same(rv.flip(0), ref.cached(v, bits), torch.float32)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("H,D,page,T", [(256, 32, 32, 130), (256, 64, 16, 131), (128, 96, 64, 257), (64, 128, 16, 520), (64, 160, 48, 515),
+                                        (32, 192, 16, 1030), (32, 224, 32, 1025), (32, 256, 128, 1041)])
+def test_many_tokens(H, D, page, T, bits, dtype):
+    """Prompts of several sequences, which start at and inside chunks of 16 in shuffled pages, a few tokens passed
+    over, and some alone in their pages."""
+    pages = -(-T // page) + 9
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(T))
+    at = torch.arange(T)
+    slots = order[at // page] * page + at % page
+    cut = T // 3 + 5  # the rest starts inside a page, out of step with the chunks
+    slots[cut:] = (at[cut:] - cut + 3) % page + order[3 + (at[cut:] - cut + 3) // page + cut // page] * page
+    slots[-3:] = order[-3:] * page + torch.tensor([0, 7, 15])
+    slots[cut + 40:cut + 43] = -1
+    k, v = some((T, H, D), dtype, T), some((T, H, D), dtype, T + 1)
+    big, small = ops.KvCache(pages, page, H, D, bits=bits), ops.KvCache(pages, page, H, D, bits=bits)
+    ops.gpu_kv_cache_write(big, k, v, slots.cuda())
+    for i in range(0, T, 16):  # the same in pieces
+        ops.gpu_kv_cache_write(small, k[i:i + 16], v[i:i + 16], slots[i:i + 16].cuda())
+    assert torch.equal(big.data, small.data)
+    rk, rv = ops.gpu_kv_cache_read(big, slots.cuda(), dtype=dtype)
+    parts = [ops.gpu_kv_cache_read(big, slots[i:i + 16].cuda(), dtype=dtype) for i in range(0, T, 16)]
+    assert torch.equal(rk, torch.cat([x[0] for x in parts])) and torch.equal(rv, torch.cat([x[1] for x in parts]))
+    rows, heads = torch.cat([torch.arange(0, 20), torch.arange(cut - 2, cut + 50), torch.arange(T - 8, T)]), torch.arange(3, H, 11)
+    gone = (slots[rows] < 0).numpy()
+    for got, x in ((rk, k), (rv, v)):
+        want = ref.cached(x[rows.cuda()][:, heads.cuda()], bits)
+        want[gone] = 0
+        same(got[rows.cuda()][:, heads.cuda()], want, dtype)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_every_code_tie_and_scale_limit(bits):
     grid = ref.GRID[bits]
