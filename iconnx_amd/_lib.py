@@ -55,7 +55,7 @@ class TokenLinear(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p), ("x_scale", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("M", ctypes.c_size_t),
                 ("K", ctypes.c_size_t), ("N", ctypes.c_size_t), ("packed", ctypes.c_void_p), ("w_scale", ctypes.c_void_p),
                 ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("x_dtype", ctypes.c_int32),
-                ("y_dtype", ctypes.c_int32)]
+                ("y_dtype", ctypes.c_int32), ("x_padded", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class KvAttention(ctypes.Structure):
@@ -123,7 +123,7 @@ SIGNATURES = {
     "icx_attention_f32": ([P, P, P, P, S, S, S, S, S, S, S, S, ctypes.c_float, I, I, P], I),
     "icx_token_weight_bytes": ([S, S], S),
     "icx_pack_token_weight": ([P, P, S, S, P], I),
-    "icx_quantize_tokens": ([P, P, I, S, S, LL, P, P], I),
+    "icx_quantize_tokens": ([P, P, I, S, S, LL, P, LL, P], I),
     "icx_token_qlinear_workspace_size": ([S, S, S, I], S),
     "icx_token_qlinear": ([P, P, P, S], I),
     "icx_kv_cache_bytes": ([P], S),

@@ -708,16 +708,18 @@ extern "C" int icx_pack_token_weight(icx_stream_t stream, const int8_t* b, size_
 }
 
 extern "C" int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dtype, size_t M, size_t K, int64_t x_stride, int8_t* q,
-                                   float* scale) {
+                                   int64_t q_stride, float* scale) {
     icx::clear_error();
     const char* who = "QuantizeTokens";
     int rc = check_sizes(M, K, 0, who);
     if (rc) return rc;
     if (!icx::is_float_kind(x_dtype))
         ICX_FAIL(ICX_ERR_DTYPE, "%s: dtype %d unsupported (must be Float32, Float16 or BFloat16)", who, x_dtype);
+    if (q_stride < (int64_t)K) ICX_FAIL(ICX_ERR_SHAPE, "%s: rows of %zu bytes at a stride of %lld", who, K, (long long)q_stride);
     if (M == 0) return ICX_OK;
     if (!x || !q || !scale) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null x, q or scale", who);
-    return quantize((hipStream_t)stream, x, x_dtype, M, K, x_stride, q, K, K, scale);
+    const size_t fill = (size_t)q_stride >= padded(K) ? padded(K) : K;
+    return quantize((hipStream_t)stream, x, x_dtype, M, K, x_stride, q, (size_t)q_stride, fill, scale);
 }
 
 extern "C" size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N, int x_dtype) {
@@ -744,11 +746,11 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* ar
     if (M == 0 || N == 0) return ICX_OK;
     if (!a.x || !a.packed || !a.w_scale || !a.y) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null x, weight, scale or y", who);
     if (!icx::aligned16(a.packed)) ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: the packed weight must be 16-byte aligned", who);
-    const bool pad = !own && K % kAlignK;
+    const bool pad = !own && K % kAlignK && !a.x_padded;
     if (!own && !pad && (a.x_stride % 16 || !icx::aligned16(a.x)))
         ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: Int8 rows of whole 128 bytes must stand at multiples of 16", who);
     const Workspace L = workspace(M, K, a.x_dtype);
-    if (L.total && (!ws || ws_bytes < L.total))
+    if ((own || pad) && L.total && (!ws || ws_bytes < L.total))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, L.total, ws_bytes);
     const hipStream_t s = (hipStream_t)stream;
     ProductArgs g{};

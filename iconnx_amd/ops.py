@@ -609,8 +609,15 @@ def _rows(x):
         ld, one = x.stride()
         if one == 1:
             return x.shape[0], ld, x
-    x = _dense(x)
     K = x.shape[-1]
+    if not x.is_contiguous():
+        try:
+            x = x.view(-1, K)  # leading axes one behind the other, rows anywhere
+            if x.stride(1) == 1:
+                return x.shape[0], x.stride(0), x
+        except RuntimeError:
+            pass
+        x = x.contiguous()
     return (x.numel() // K if K else 0), K, x
 
 
@@ -645,7 +652,8 @@ class TokenWeight:
 def gpu_quantize_tokens(x):
     """(q int8 of x's shape, scale float32 [...]) of x [..., K]: for each token the scale
     max(max|x| / 127, 2^-126) and q = x / scale rounded to nearest even.  A token that is not finite
-    throughout has the scale NaN and zeros."""
+    throughout has the scale NaN and zeros.  Tokens of q stand at multiples of 128 bytes, as the products
+    read them: where K is none, q is a slice of a wider tensor."""
     who = "QuantizeTokens"
     code = _float_code(x.dtype, who)
     shape = x.shape
@@ -655,14 +663,16 @@ def gpu_quantize_tokens(x):
     M, ld, x = _rows(x)
     dev = x.device
     shape = tuple(shape)  # (as a tuple: torch.empty takes a Size half as fast)
-    q = _empty(shape, dtype=_I8, device=dev)
+    K = shape[-1]
+    Kp = K + -K % 128
+    q = _empty(shape[:-1] + (Kp,), dtype=_I8, device=dev)
     scale = _empty(shape[:-1], dtype=_F32, device=dev)
-    check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, shape[-1], ld, q.data_ptr(), scale.data_ptr()))
-    return q, scale
+    check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, K, ld, q.data_ptr(), Kp, scale.data_ptr()))
+    return (q if Kp == K else q[..., :K]), scale
 
 
 # (arguments by struct: packing thirteen values costs a fifth of converting them one by one)
-_LINEAR_PACK = struct.Struct("=QQqQQQQQQQqii")
+_LINEAR_PACK = struct.Struct("=QQqQQQQQQQqiiii")
 assert _LINEAR_PACK.size == ctypes.sizeof(TokenLinear)
 
 
@@ -703,10 +713,17 @@ def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
             raise IconnxError(ERR_SHAPE, "%s: out must be a contiguous %s %s" % (who, _name(yt), list(oshape)))
         _on_device(who, here, out)
     M, ld, x = _rows(x)
-    if code == ICX_I8 and K % 128 == 0 and (ld | x.data_ptr()) % 16:  # rows that the products cannot read in place
-        ld, x = K, x.clone(memory_format=torch.contiguous_format)
+    padded = 0
+    if code == ICX_I8:
+        odd = (ld | x.data_ptr()) % 16
+        if K % 128 == 0:
+            if odd:  # rows that the products cannot read in place
+                ld, x = K, x.clone(memory_format=torch.contiguous_format)
+        elif not odd:  # (in place if the last row's storage goes on as far as they read)
+            Kp = K + -K % 128
+            padded = int(ld >= Kp and x.storage_offset() + (M - 1) * ld + Kp <= x.untyped_storage().nbytes())
     L = lib()
-    nws = w._ws.get((M, code))
+    nws = 0 if padded else w._ws.get((M, code))
     if nws is None:
         if len(w._ws) > 4096:  # (a size for each number of tokens that came by)
             w._ws.clear()
@@ -715,7 +732,7 @@ def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
         out = x.new_empty(oshape) if yt == x.dtype else _empty(oshape, dtype=yt, device=x.device)
     ws = _empty(nws, dtype=_U8, device=x.device) if nws else None
     args = _LINEAR_PACK.pack(x.data_ptr(), 0 if x_scale is None else x_scale.data_ptr(), ld, M, K, N, w.packed.data_ptr(),
-                             w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), N, code, ycode)
+                             w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), N, code, ycode, padded, 0)
     check(L.icx_token_qlinear(_stream(), args, None if ws is None else ws.data_ptr(), nws))
     return out
 

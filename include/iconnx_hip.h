@@ -343,13 +343,15 @@ int icx_attention_f32(icx_stream_t stream, const float* q, const float* k, const
  * The weight, int8 [K, N], is packed once into icx_token_weight_bytes (16-byte aligned). */
 size_t icx_token_weight_bytes(size_t K, size_t N);
 int icx_pack_token_weight(icx_stream_t stream, const int8_t* b, size_t K, size_t N, int8_t* packed);
-/* q [M, K] dense and scale [M] of x [M, K] (row stride x_stride). */
+/* q [M, K] (row stride q_stride; where that reaches the next multiple of 128, zeros up to there) and scale
+ * [M] of x [M, K] (row stride x_stride). */
 int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dtype, size_t M, size_t K, int64_t x_stride, int8_t* q,
-                        float* scale);
+                        int64_t q_stride, float* scale);
 /* x [M, K]: ICX_I8 with x_scale [M] (icx_quantize_tokens' outputs, for several products over one input),
- * or a float type with x_scale NULL, quantized on the way.  Int8 rows of whole 128 bytes (K % 128 == 0)
- * are read in place and have to stand at multiples of 16 bytes (ICX_ERR_INVALID_ARG).  y [M, N]; bias [N]
- * f32 or NULL.  The workspace may be 0. */
+ * or a float type with x_scale NULL, quantized on the way.  Int8 rows of whole 128 bytes (K % 128 == 0), or
+ * behind which memory may be read up to the next multiple of 128 (x_padded 1; whatever it holds), are
+ * read in place and have to stand at multiples of 16 bytes (ICX_ERR_INVALID_ARG); others are copied.
+ * y [M, N]; bias [N] f32 or NULL.  The workspace may be 0. */
 typedef struct icx_token_linear {
     const void* x;
     const float* x_scale;
@@ -361,6 +363,7 @@ typedef struct icx_token_linear {
     void* y;
     int64_t y_stride;
     int32_t x_dtype, y_dtype;
+    int32_t x_padded, reserved;
 } icx_token_linear;
 size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N, int x_dtype);
 int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* args, void* workspace, size_t workspace_bytes);

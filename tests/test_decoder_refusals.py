@@ -84,7 +84,7 @@ def test_cache_writes_and_reads_that_are_refused(L):
 
 def test_products_that_are_refused(L):
     def run(x=PTR, xt=BF16, xs=None, M=2, K=64, N=32, w=PTR, ws=PTR, y=PTR, yt=F32, work=None, n=0, ld=None):
-        args = _lib.TokenLinear(x, xs, K if ld is None else ld, M, K, N, w, ws, None, y, N, xt, yt)
+        args = _lib.TokenLinear(x, xs, K if ld is None else ld, M, K, N, w, ws, None, y, N, xt, yt, 0, 0)
         return L.icx_token_qlinear(None, ctypes.byref(args), work, n)
 
     assert L.icx_token_qlinear(None, None, None, 0) == BAD
@@ -101,7 +101,8 @@ def test_products_that_are_refused(L):
     assert run(M=2000, work=PTR, n=need - 1) == WORKSPACE and run(M=2000, n=need) == WORKSPACE
     assert L.icx_token_weight_bytes(100, 7) == 128 * 7
     assert L.icx_pack_token_weight(None, None, 64, 32, PTR) == BAD and L.icx_pack_token_weight(None, PTR, 0, 32, PTR) == SHAPE
-    assert L.icx_quantize_tokens(None, PTR, I8, 1, 64, 64, PTR, PTR) == DTYPE
-    assert L.icx_quantize_tokens(None, PTR, F32, 1, 0, 64, PTR, PTR) == SHAPE
-    assert L.icx_quantize_tokens(None, None, F32, 1, 64, 64, PTR, PTR) == BAD
-    assert L.icx_quantize_tokens(None, None, F32, 0, 64, 64, None, None) == 0
+    assert L.icx_quantize_tokens(None, PTR, I8, 1, 64, 64, PTR, 64, PTR) == DTYPE
+    assert L.icx_quantize_tokens(None, PTR, F32, 1, 0, 64, PTR, 64, PTR) == SHAPE
+    assert L.icx_quantize_tokens(None, None, F32, 1, 64, 64, PTR, 64, PTR) == BAD
+    assert L.icx_quantize_tokens(None, PTR, F32, 1, 64, 64, PTR, 63, PTR) == SHAPE
+    assert L.icx_quantize_tokens(None, None, F32, 0, 64, 64, None, 64, None) == 0

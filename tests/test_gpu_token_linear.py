@@ -118,6 +118,15 @@ def test_rows_with_a_stride_an_offset_and_leading_axes(M, K, N):
     wide = torch.zeros(M, K + 3, dtype=torch.int8, device="cuda")
     wide[:, 3:] = qa
     assert torch.equal(ops.gpu_token_qlinear(wide[:, 3:], tw, x_scale=sa, dtype=torch.bfloat16), want)
+    # int8 rows whose storage ends with the last of them, and goes on behind it
+    for tail in (0, 5, 128):
+        flat = torch.full(((M - 1) * 512 + K + tail + 16,), 77, dtype=torch.int8, device="cuda")
+        rows = torch.as_strided(flat, (M, K), (512, 1), 16)
+        rows.copy_(qa)
+        assert torch.equal(ops.gpu_token_qlinear(rows, tw, x_scale=sa, dtype=torch.bfloat16), want)
+    three, s3 = ops.gpu_quantize_tokens(part.contiguous().view(2, M // 2, K))
+    assert three.shape == (2, M // 2, K) and torch.equal(three.reshape(M, K), qa)
+    assert torch.equal(ops.gpu_token_qlinear(three, tw, x_scale=s3, dtype=torch.bfloat16).view(M, N), want)
     out = torch.empty_like(want)
     assert ops.gpu_token_qlinear(part, tw, out=out) is out and torch.equal(out, want)
 
