@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) kv_attention_join_kernel(Attn
     const int64_t at = (int64_t)token * a.heads_q + hq;
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (lane < a.splits) ml = a.ml[lane * all + at];
-    // over as many lanes as there are shares: each exchange costs as much as a load from L2 takes to start
+    // over as many lanes as there are shares: the exchanges wait for one another
     const int half = a.splits > 1 ? 1 << (31 - __builtin_clz(a.splits - 1)) : 0;
     float top = ml.x;
     for (int off = half; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
@@ -101,21 +101,26 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     p.few_rows = many && (a.batch == 1 || (size_t)a.rows * group > 2 * kFewRows * a.batch) ? 0 : (int)kFewRows;
     p.row_tiles = (int)icx::cdiv(std::min(most, (size_t)p.few_rows), 16);
     // Tiles of all sequences together: each may end in a part of one.  Blocks of 8 waves decode a token half as
-    // often, and are taken where they still give every CU one: WIDE.
-    const int G = c.head_size / 32;
+    // often, but wait for one another and fill the CUs in coarser steps.  They are taken for long caches, where
+    // they still give every CU one: rows over tokens, us, in 8 and in 4 waves, 32 bfloat16 heads over 8 of 128:
+    // 16384 over 16384 2193 and 2350, 4 times 1024 over 8192 273 and 283, but 16 times 2048 over 2048 421 and 410
+    // and 32 times 512 over 1024 153 and 139.
+    const int G = c.head_size / 32, terms = icx::attention_terms(a.dtype);
+    const size_t tokens = (size_t)a.table_width * c.page_size;
     size_t tiles = 0;
     p.tile_waves = 4;
     for (int waves : {8, 4}) {
-        if (!many || (waves == 8 && G > icx::kWideHeads)) continue;
-        const size_t tile = 16 * waves * (size_t)icx::attention_wave_tiles(G, icx::attention_terms(a.dtype));
+        if (!many || (waves == 8 && (tokens < 4096 || !icx::attention_wide(G, terms)))) continue;
+        const size_t tile = 16 * waves * (size_t)icx::attention_wave_tiles(G, terms);
         tiles = std::min((size_t)a.batch * icx::cdiv(most, tile), icx::cdiv((size_t)a.rows * group, tile) + a.batch);
         p.tile_waves = waves;
         if (c.kv_heads * icx::cdiv((size_t)a.rows * group, tile) >= (size_t)icx::num_cus()) break;
     }
     const size_t full = many ? c.kv_heads * tiles : heads * p.row_tiles;
-    const size_t tokens = (size_t)a.table_width * c.page_size;
-    const size_t want = many ? (size_t)icx::num_cus() * 8 / p.tile_waves / std::max<size_t>(full, 1)
-                             : icx::cdiv((size_t)icx::num_cus() * 8, std::max<size_t>(full, 1));
+    // Shares, to fill the CUs.  For few rows with up to 3 blocks of them a CU: against 8 a CU, 46.2 us for 54.6 at 8
+    // sequences of 32768 tokens (4 bits, 32 heads over 8 of 128), 23.8 for 36.3 at 4 of 16384, 28.6 for 33.7 at 32
+    // of 4096; against 1, 70.1, 25.0 and 35.6.
+    const size_t want = (many ? (size_t)icx::num_cus() * 8 / p.tile_waves : (size_t)icx::num_cus() * 3) / std::max<size_t>(full, 1);
     p.splits = (int)std::max<size_t>(1, std::min({want, icx::cdiv(tokens, 256), (size_t)kMaxSplits}));
     p.few = heads * p.row_tiles * p.splits;
     p.many = c.kv_heads * tiles * p.splits;

@@ -39,7 +39,7 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
     Sequence s;
     s.start = a.starts ? a.starts[b] : b;
     int n = 0;
-    if (s.start >= 0 && s.start <= a.rows_total) n = a.starts ? max(0, min(a.starts[b + 1], a.rows_total) - s.start) : 1;
+    if (s.start >= 0 && s.start <= a.rows_total) n = a.starts ? max(0, min(max(a.starts[b + 1], 0), a.rows_total) - s.start) : 1;
     s.rows = min(n, a.max_rows);
     s.len = max(0, min(a.lengths[b], a.width * a.page_size));
     s.base = s.len - n;
@@ -52,8 +52,10 @@ constexpr int attention_terms(int dtype) { return dtype == ICX_BF16 ? 1 : dtype 
 // Tiles of 16 rows of a wave of kv_attention_tiles_kernel: two while their queries and sums fit the
 // registers.
 constexpr int attention_wave_tiles(int G, int terms) { return G * terms >= 12 ? 1 : 2; }
-// Its blocks are of 4 waves, or for heads of up to 32 times this of 8 (LDS holds no more of two steps).
-constexpr int kWideHeads = 4;
+// Its blocks are of 4 waves, or for bfloat16 heads of up to 128 of 8.  (LDS holds no more of two steps.  float16
+// and float32 gain nothing from 8: 16384 rows over as many tokens 3710 us for 3503, and 5377 for 5501, 2 times
+// 4096 over 8192 981 for 853, and 1222 for 1190.)
+constexpr bool attention_wide(int G, int terms) { return G <= 4 && terms == 1; }
 
 void launch_attention_bf16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);
 void launch_attention_f16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);

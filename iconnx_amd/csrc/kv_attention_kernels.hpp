@@ -801,7 +801,7 @@ void launch_heads(unsigned few, unsigned many, hipStream_t s, const AttnArgs& a)
         const size_t lds = kWaves * held * (32 * G + 4) * 4 + kWaves * 16 * 8;
         kv_attention_rows_kernel<BITS, TERMS, G, T><<<few, 64 * kWaves, lds, s>>>(a);
     }
-    if constexpr (G <= icx::kWideHeads) {
+    if constexpr (icx::attention_wide(G, TERMS)) {
         if (many && a.tile_waves == 8) {
             kv_attention_tiles_kernel<BITS, TERMS, G, 8, T><<<many, 512, 0, s>>>(a);
             return;
