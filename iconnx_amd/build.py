@@ -20,10 +20,15 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 #   reference's separate ONNX nodes do.
 # -fhip-fp32-correctly-rounded-divide-sqrt: IEEE f32 division in the Div epilogue op.
 # -packed-fp32-ops disabled: no v_pk_*_f32 generation.
+# -amdgpu-remove-redundant-endcf=false: every branch that lanes take apart restores their mask at its own end.
+#   Left out where an outer branch ends at the same place, a register that was put aside can come back in
+#   between, for the inner branch's lanes alone: attention rows of 256-value heads were stored from the wrong
+#   address by the other lanes.
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall",
     "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    "-mllvm", "-amdgpu-remove-redundant-endcf=false",
 ]
 # host-only C++ (the graph executor) goes through hipcc for the HIP runtime headers
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall"]
