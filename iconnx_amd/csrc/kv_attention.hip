@@ -1,6 +1,7 @@
 // The attention's entry point and the kernel that joins shares of the tokens; the attention itself is in
 // kv_attention_kernels.hpp.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "internal.hpp"
@@ -93,7 +94,7 @@ struct Plan {
 constexpr size_t kFewRows = 32;
 Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     Plan p;
-    const size_t group = (size_t)(a.q_heads / c.kv_heads), most = (size_t)a.max_rows * group;
+    const size_t group = (size_t)(a.q_heads / c.kv_heads), most = (size_t)std::min(a.max_rows, a.rows) * group;
     const size_t heads = (size_t)a.batch * c.kv_heads;
     const bool many = most > kFewRows;
     // Beside sequences of many rows, those of few have a kernel of their own where they may well be most of
@@ -146,8 +147,15 @@ int check_attention(const icx_kv_cache* c, const icx_kv_attention* a, const char
                  (long long)a->table_width * c->page_size, a->rows);
     if (!a->q_starts && a->rows != a->batch)
         ICX_FAIL(ICX_ERR_SHAPE, "%s: without q_starts there is one row a sequence (%d rows, %d sequences)", who, a->rows, a->batch);
+    if ((int64_t)a->rows * a->q_heads > 0x7fffffff)
+        ICX_FAIL(ICX_ERR_SHAPE, "%s: %d rows of %d heads are too many", who, a->rows, a->q_heads);
     if (!(a->softcap >= 0.0f) || a->window < 0)
         ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: softcap %g and window %d must not be negative", who, (double)a->softcap, a->window);
+    // (past 2^64 what a score is worth in the cap's units is not a normal number for every scale; past 1024 the
+    // short form of tanh is not close enough for a score far below the cap)
+    const float most = a->dtype == ICX_F32 ? 0x1p64f : 1024.0f;
+    if (a->softcap > most && !std::isinf(a->softcap))
+        ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: softcap %g (must be up to %g for this dtype, or infinite)", who, (double)a->softcap, (double)most);
     return ICX_OK;
 }
 
@@ -170,7 +178,7 @@ extern "C" int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* c
     if (!args->q || !args->out || !args->lengths || (!args->page_table && args->table_width))
         ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: null q, out, page_table or lengths", who);
     const Plan p = plan_of(*cache, *args);
-    if ((p.few | p.many) > 0xffffffull || (uint64_t)args->rows * 64 * kJoinWaves > 0xffffffffull)
+    if (std::max(p.few, p.many) > 0x7fffffull || (uint64_t)args->rows * 64 * kJoinWaves > 0xffffffffull)
         ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %d sequences of up to %d rows are too many for a launch", who, args->batch, args->max_rows);
     if (p.part_bytes && (!ws || ws_bytes < p.part_bytes + p.ml_bytes))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, p.part_bytes + p.ml_bytes, ws_bytes);
@@ -193,10 +201,10 @@ extern "C" int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* c
     a.batch = args->batch;
     a.group = args->q_heads / cache->kv_heads;
     a.heads_q = args->q_heads;
-    a.max_rows = args->max_rows;
+    a.max_rows = std::min(args->max_rows, args->rows);
     a.rows_total = args->rows;
     a.scale = args->scale;
-    a.softcap = args->softcap;
+    a.softcap = std::isinf(args->softcap) ? 0.0f : args->softcap;
     a.window = args->window < args->table_width * cache->page_size ? args->window : 0;  // 0: every token
     a.causal = args->causal;
     a.slopes = args->slopes;

@@ -56,7 +56,9 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[TER
 }
 
 // cap tanh(x), x given in units of log2(e) / 2: through exp2, and in float32 (TERMS 3) by its series near 0,
-// where that form's error, 2^-22 of the cap, is not below a score's own any more.
+// where that form's error, 2^-22 of the cap, is not below a score's own any more.  (The other types' caps end at
+// 1024, where the error is half of float16's rounding of the weight; with the series in them too, for larger
+// ones, the registers do not hold the rest: 4096 rows over 8192 tokens 460 us for 390.)
 template <int TERMS>
 __device__ __forceinline__ float capped(float x, float cap) {
     const float e = __builtin_amdgcn_exp2f(x);

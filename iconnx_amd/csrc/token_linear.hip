@@ -682,6 +682,7 @@ Workspace workspace(size_t M, size_t K, int x_dtype) {
 
 // The sums stay within 32 bits: |w|, |q| <= 128.
 constexpr size_t kMaxK = 131071;
+constexpr int64_t kMaxStride = (int64_t)1 << 23;
 
 int check_sizes(size_t M, size_t K, size_t N, const char* who) {
     if (K < 1 || K > kMaxK) ICX_FAIL(ICX_ERR_SHAPE, "%s: K = %zu (must be 1 to %zu)", who, K, kMaxK);
@@ -749,6 +750,9 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* ar
     const bool pad = !own && K % kAlignK && !a.x_padded;
     if (!own && !pad && (a.x_stride % 16 || !icx::aligned16(a.x)))
         ICX_FAIL(ICX_ERR_INVALID_ARG, "%s: Int8 rows of whole 128 bytes must stand at multiples of 16", who);
+    // (a tile's rows are reached by offsets of 32 bits)
+    if (!own && !pad && (a.x_stride < 0 || a.x_stride > kMaxStride))
+        ICX_FAIL(ICX_ERR_SHAPE, "%s: Int8 rows at a stride of %lld (must be up to %lld)", who, (long long)a.x_stride, (long long)kMaxStride);
     const Workspace L = workspace(M, K, a.x_dtype);
     if ((own || pad) && L.total && (!ws || ws_bytes < L.total))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, L.total, ws_bytes);

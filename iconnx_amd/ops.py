@@ -638,11 +638,20 @@ class TokenWeight:
         _on_device(who, _here(), b, scale)
         b = _dense(b)
         self.K, self.N = b.shape
-        self.scale = scale.contiguous()
+        self._scale = scale.contiguous()
         L = lib()
-        self.packed = _empty(L.icx_token_weight_bytes(self.K, self.N), dtype=_I8, device=b.device)
-        check(L.icx_pack_token_weight(_stream(), b.data_ptr(), self.K, self.N, self.packed.data_ptr()))
-        self._device, self._ws = self.packed.get_device(), {}
+        self._packed = _empty(L.icx_token_weight_bytes(self.K, self.N), dtype=_I8, device=b.device)
+        check(L.icx_pack_token_weight(_stream(), b.data_ptr(), self.K, self.N, self._packed.data_ptr()))
+        self._device, self._ws = self._packed.get_device(), {}
+
+    # (not to be set: the products take their addresses and sizes as they are)
+    @property
+    def scale(self):
+        return self._scale
+
+    @property
+    def packed(self):
+        return self._packed
 
     @property
     def shape(self):
@@ -717,9 +726,9 @@ def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
     if code == ICX_I8:
         odd = (ld | x.data_ptr()) % 16
         if K % 128 == 0:
-            if odd:  # rows that the products cannot read in place
+            if odd or ld > 1 << 23:  # rows that the products cannot read in place
                 ld, x = K, x.clone(memory_format=torch.contiguous_format)
-        elif not odd:  # (in place if the last row's storage goes on as far as they read)
+        elif not odd and ld <= 1 << 23:  # (in place if the last row's storage goes on as far as they read)
             Kp = K + -K % 128
             padded = int(ld >= Kp and x.storage_offset() + (M - 1) * ld + Kp <= x.untyped_storage().nbytes())
     L = lib()
@@ -731,8 +740,8 @@ def gpu_token_qlinear(x, w, x_scale=None, bias=None, dtype=None, out=None):
     if out is None:
         out = x.new_empty(oshape) if yt == x.dtype else _empty(oshape, dtype=yt, device=x.device)
     ws = _empty(nws, dtype=_U8, device=x.device) if nws else None
-    args = _LINEAR_PACK.pack(x.data_ptr(), 0 if x_scale is None else x_scale.data_ptr(), ld, M, K, N, w.packed.data_ptr(),
-                             w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), N, code, ycode, padded, 0)
+    args = _LINEAR_PACK.pack(x.data_ptr(), 0 if x_scale is None else x_scale.data_ptr(), ld, M, K, N, w._packed.data_ptr(),
+                             w._scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), N, code, ycode, padded, 0)
     check(L.icx_token_qlinear(_stream(), args, None if ws is None else ws.data_ptr(), nws))
     return out
 
@@ -749,11 +758,16 @@ class KvCache:
         n = lib().icx_kv_cache_bytes(ctypes.byref(self._desc))
         if not n:
             raise IconnxError(ERR_UNSUPPORTED, lib().icx_last_error().decode())
-        self.data = torch.zeros(n, dtype=_U8, device=device)
-        _require_cuda(self.data)
-        self._desc.data = self.data.data_ptr()
-        self._device, self._heads = self.data.get_device(), (kv_heads, head_size)
+        self._data = torch.zeros(n, dtype=_U8, device=device)
+        _require_cuda(self._data)
+        self._desc.data = self._data.data_ptr()
+        self._device, self._heads = self._data.get_device(), (kv_heads, head_size)
         self._as_parameter_ = ctypes.addressof(self._desc)  # what a pointer argument takes when given the cache
+
+    @property
+    def data(self):
+        """The cache's bytes (uint8); the tensor may be filled, as from a copy, but not exchanged for another."""
+        return self._data
 
 
 def _check_slots(slots, who):
@@ -771,7 +785,8 @@ assert _WRITE_PACK.size == ctypes.sizeof(KvWrite)
 
 def gpu_kv_cache_write(cache, k, v, slots):
     """Quantizes k and v [tokens, kv_heads, head_size] (any strides with dense heads) into the cache's
-    ``slots`` [tokens]; a slot outside the cache, as -1, is passed over."""
+    ``slots`` [tokens]; a slot outside the cache, as -1, is passed over.  No slot may come twice (it would hold
+    codes of both tokens)."""
     who = "KvCacheWrite"
     code = _float_code(k.dtype, who)
     if v.dtype != k.dtype:
@@ -825,7 +840,8 @@ def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_row
     int32 [batch + 1], the rows q_starts[b] .. q_starts[b + 1] - 1 are the last tokens of sequence b, at
     most ``max_rows`` of each (by default all).  heads is a multiple of the cached heads.  A row at position
     p sees the tokens j <= p (``causal``) and j > p - ``window`` (0: all); scores are q.k ``scale``
-    (head_size ** -0.5), through softcap tanh(. / ``softcap``) if that is given, plus ``slopes``[head]
+    (head_size ** -0.5), through softcap tanh(. / ``softcap``) if that is given (up to 1024, float32 2^64; infinite:
+    none), plus ``slopes``[head]
     (j - p), float32.  A row that sees no token is zero; rows of ``out`` past q_starts[batch] keep what they held."""
     who = "KvCacheAttention"
     code = _float_code(q.dtype, who)

@@ -350,7 +350,8 @@ int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dtype, size_t 
 /* x [M, K]: ICX_I8 with x_scale [M] (icx_quantize_tokens' outputs, for several products over one input),
  * or a float type with x_scale NULL, quantized on the way.  Int8 rows of whole 128 bytes (K % 128 == 0), or
  * behind which memory may be read up to the next multiple of 128 (x_padded 1; whatever it holds), are
- * read in place and have to stand at multiples of 16 bytes (ICX_ERR_INVALID_ARG); others are copied.
+ * read in place and have to stand at multiples of 16 bytes (ICX_ERR_INVALID_ARG), at most 2^23 apart
+ * (ICX_ERR_SHAPE); others are copied.
  * y [M, N]; bias [N] f32 or NULL.  The workspace may be 0. */
 typedef struct icx_token_linear {
     const void* x;
@@ -383,7 +384,8 @@ typedef struct icx_kv_cache {
 size_t icx_kv_cache_bytes(const icx_kv_cache* cache); /* 0 for a cache that is not supported */
 /* Quantizes k, v [tokens, kv_heads, head_size] (token and head strides given) into the slots
  * (page * page_size + place in it; ICX_I32 or ICX_I64, on the device).  A slot outside the cache, as a
- * negative one, is passed over.  A slot named twice in one call keeps codes of either token. */
+ * negative one, is passed over.  A slot named twice in one call is left with codes of both tokens in no
+ * order, and harms no other slot. */
 typedef struct icx_kv_write {
     const void* k;
     const void* v;
@@ -405,7 +407,8 @@ int icx_kv_cache_read(icx_stream_t stream, const icx_kv_cache* cache, const void
  * NULL; at most max_rows rows of a sequence are done.  Query head h reads cached head
  * h / (q_heads / kv_heads).  Row i of n stands at p = lengths[b] - n + i:
  *   out = softmax_j(cap(scale q.k_j) + slopes[h] (j - p)) v_j  over  j <= p (causal) and j > p - window
- * (window 0: no limit), cap(s) = softcap tanh(s / softcap) (softcap 0: none), slopes [q_heads] f32 or
+ * (window 0: no limit), cap(s) = softcap tanh(s / softcap) (softcap 0 or infinite: none; otherwise up
+ * to 1024, in ICX_F32 2^64), slopes [q_heads] f32 or
  * NULL.  A row that sees no token is zero; tokens in a page outside the cache are not seen.  Rows of
  * out that belong to no sequence are left as they were. */
 typedef struct icx_kv_attention {

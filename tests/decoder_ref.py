@@ -90,8 +90,10 @@ def attention(q, k, v, lengths, starts, scale, softcap=0.0, window=0, slopes=Non
                 s = kk @ q[r, h] * scale
                 d = (terms * D + 8) * a + 4 * np.abs(s)
                 if softcap:
+                    # (in float32 the roundings are a score's own: 6 of its series, or 8 of the cap where that
+                    # is no more than four times the score)
+                    d = d + 8 * (softcap if terms < 3 else np.minimum(softcap, 4 * np.abs(s)))
                     s = softcap * np.tanh(s / softcap)
-                    d = d + softcap * 8
                 if slopes is not None:
                     t = slopes[h] * (jj - p)
                     s = s + t

@@ -53,6 +53,8 @@ def attention(**kw):
 @pytest.mark.parametrize("kw,status", [(dict(dtype=I8), DTYPE), (dict(q_heads=3), SHAPE), (dict(q_heads=0), SHAPE), (dict(rows=-1), SHAPE),
                                        (dict(batch=4), SHAPE), (dict(max_rows=-2), SHAPE), (dict(table_width=-1), SHAPE),
                                        (dict(table_width=1 << 27), SHAPE), (dict(softcap=-1.0), BAD), (dict(softcap=float("nan")), BAD),
+                                       (dict(softcap=1e20), UNSUPPORTED), (dict(softcap=1025.0, dtype=BF16), UNSUPPORTED),
+                                       (dict(softcap=1025.0, dtype=F16), UNSUPPORTED), (dict(rows=1 << 20, batch=1, q_starts=PTR, q_heads=4096), SHAPE),
                                        (dict(window=-1), BAD), (dict(q=None), BAD), (dict(out=None), BAD), (dict(lengths=None), BAD),
                                        (dict(page_table=None), BAD), (dict(table_width=1 << 20), WORKSPACE)])
 def test_attention_that_is_refused(L, kw, status):
@@ -89,6 +91,7 @@ def test_products_that_are_refused(L):
 
     assert L.icx_token_qlinear(None, None, None, 0) == BAD
     assert run(xt=I8, xs=PTR, K=128, x=PTR + 1) == BAD and run(xt=I8, xs=PTR, K=128, ld=130) == BAD
+    assert run(xt=I8, xs=PTR, K=128, ld=(1 << 23) + 16) == SHAPE and run(xt=I8, xs=PTR, K=128, ld=-128) == SHAPE
     assert run(xt=I8, xs=PTR, K=100) == WORKSPACE  # (rows that have to be padded)
 
     assert run(xt=I32) == DTYPE and run(yt=I8) == DTYPE

@@ -270,6 +270,27 @@ def test_long_sequences(lengths, rows, dtype):
     f.check(query(n, 4, 64, dtype), rows, window=777)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [None, [3, 50]])
+def test_caps_far_above_the_scores(rows, dtype):
+    """In float32 a score keeps its own precision under a cap of any size; an infinite one is none."""
+    f = Filled([100, 150], 2, 64, 16, 8)
+    q = query(2 if rows is None else sum(rows), 4, 64, dtype)
+    for cap in (65.0, 1024.0) + ((1e4, 1e7, 2.0 ** 64) if dtype == torch.float32 else ()):
+        f.check(q, rows, softcap=cap)
+    assert torch.equal(f.attend(q, rows, softcap=float("inf")), f.attend(q, rows))
+
+
+def test_more_rows_are_allowed_than_there_are():
+    f = Filled([40] * 8, 1, 64, 16, 8)
+    q = query(8, 8, 64, torch.bfloat16)
+    want = f.attend(q)
+    for most in (8, 1 << 29, 2 ** 31 - 1):
+        assert torch.equal(f.attend(q, [1] * 8, max_rows=most), f.attend(q, [1] * 8, max_rows=8))
+    f.check(q, [1] * 8, max_rows=1 << 29)
+    assert torch.equal(f.attend(q, [1] * 8, max_rows=1), want)
+
+
 @pytest.mark.parametrize("rows", [[5, 0, 9], [64, 3, 70]])
 def test_more_rows_than_tokens_and_rows_behind_the_last_sequence(rows):
     """Rows that stand before the first token are zero; rows of no sequence stay as they were."""
@@ -457,6 +478,33 @@ def test_a_cache_past_four_gigabytes(rows):
                                           torch.tensor([2048], dtype=torch.int32).cuda(), q_starts=starts, window=n - 50)
 
     assert torch.equal(run(cache, pages - 2), run(small, 0))
+
+
+def test_a_cache_keeps_its_memory():
+    cache = ops.KvCache(4, 16, 2, 64)
+    with pytest.raises(AttributeError):
+        cache.data = cache.data.clone()
+    other = ops.KvCache(4, 16, 2, 64)
+    k = torch.randn(5, 2, 64).cuda()
+    slots = torch.arange(5).cuda()
+    ops.gpu_kv_cache_write(cache, k, k, slots)
+    other.data.copy_(cache.data)
+    assert torch.equal(ops.gpu_kv_cache_read(other, slots)[0], ops.gpu_kv_cache_read(cache, slots)[0])
+
+
+@pytest.mark.parametrize("T", [40, 4100])
+def test_slots_named_twice_harm_no_others(T):
+    cache = ops.KvCache(T // 16 + 2, 16, 8, 32)
+    k = torch.randn(T, 8, 32).cuda()
+    slots = torch.arange(T).cuda()
+    ops.gpu_kv_cache_write(cache, k, k, slots)
+    want = ops.gpu_kv_cache_read(cache, slots)[0]
+    twice = slots.clone()
+    twice[T - 3:] = 7
+    ops.gpu_kv_cache_write(cache, k, k, twice)
+    got = ops.gpu_kv_cache_read(cache, slots)[0]
+    keep = slots != 7
+    assert torch.equal(got[keep], want[keep])
 
 
 def test_refusals():

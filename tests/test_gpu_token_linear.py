@@ -124,6 +124,10 @@ def test_rows_with_a_stride_an_offset_and_leading_axes(M, K, N):
         rows = torch.as_strided(flat, (M, K), (512, 1), 16)
         rows.copy_(qa)
         assert torch.equal(ops.gpu_token_qlinear(rows, tw, x_scale=sa, dtype=torch.bfloat16), want)
+    # ... and whose distance passes what a tile's offsets hold
+    far = torch.zeros(3 * (1 << 24), dtype=torch.int8, device="cuda").view(3, 1 << 24)[:, :K]
+    far.copy_(qa[:3])
+    assert torch.equal(ops.gpu_token_qlinear(far, tw, x_scale=sa[:3].contiguous(), dtype=torch.bfloat16), want[:3])
     three, s3 = ops.gpu_quantize_tokens(part.contiguous().view(2, M // 2, K))
     assert three.shape == (2, M // 2, K) and torch.equal(three.reshape(M, K), qa)
     assert torch.equal(ops.gpu_token_qlinear(three, tw, x_scale=s3, dtype=torch.bfloat16).view(M, N), want)
@@ -174,3 +178,5 @@ def test_refusals():
     for f in bad:
         with pytest.raises(ops.IconnxError):
             f()
+    with pytest.raises(AttributeError):
+        tw.scale = s
