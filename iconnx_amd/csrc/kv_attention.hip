@@ -88,7 +88,7 @@ void launch_join(hipStream_t s, const AttnArgs& a) {
 
 // How the call is cut: tiles of rows and shares of the tokens.
 struct Plan {
-    int row_tiles, few_rows, splits, tile_waves;
+    int row_tiles, few_rows, splits, tile_waves, wave_tiles;
     size_t few, many, part_bytes, ml_bytes;  // blocks of either kernel, workspace
 };
 constexpr size_t kFewRows = 32;
@@ -101,28 +101,39 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     // the batch; else, and in a batch of one, the launch (4 us) costs more than it gives.
     p.few_rows = many && (a.batch == 1 || (size_t)a.rows * group > 2 * kFewRows * a.batch) ? 0 : (int)kFewRows;
     p.row_tiles = (int)icx::cdiv(std::min(most, (size_t)p.few_rows), 16);
-    // Tiles of all sequences together: each may end in a part of one.  Blocks of 8 waves decode a token half as
-    // often, but wait for one another and fill the CUs in coarser steps.  They are taken for long caches, where
-    // they still give every CU one: rows over tokens, us, in 8 and in 4 waves, 32 bfloat16 heads over 8 of 128:
-    // 16384 over 16384 2193 and 2350, 4 times 1024 over 8192 273 and 283, but 16 times 2048 over 2048 421 and 410
-    // and 32 times 512 over 1024 153 and 139.
+    // Tiles of all sequences together (each may end in a part of one) and shares of the tokens that a row may see,
+    // by the blocks that they make.  Decoding the tokens costs a block the same for 64, 128 or 256 rows of tiles;
+    // small tiles fill the CUs where large ones do not, and heads of up to 64 leave their waves registers enough to
+    // be more a CU.  us, measured with 8 bits and bfloat16 if not said otherwise, rows over tokens:
+    //  * 8 waves of 32 rows for long caches, where that makes 2 blocks a CU: 8192 over 8192, 32 heads over 8 of 128,
+    //    580 against 618 with 4 waves, of 64 379 / 422; but 16 times 256 over 4096 (1 a CU) 226 / 150, and 32 times
+    //    512 over 1024 (4 bits) 153 / 139;
+    //  * 4 waves of 32 rows if, with the shares, they make 2 blocks a CU: 8 times 300 over 3000 (4 bits) 97 against
+    //    121 with 16 rows, 2 times 256 over 8192 82 / 116; but 8 times 200 over 200 (4 bits) 16.3 / 14.7, one
+    //    sequence of 64 over 512 15.9 / 13.7, and 2 heads of 256, 512 over 2048, 45 / 41;
+    //  * 4 waves of 16 rows else, and for heads of up to 64: 12 of 64, 8 times 1024 over 1024 33.1 against 34.1 with
+    //    32 rows (float32 45.8 / 57.9), 8 times 300 over 3000 (4 bits) 44 / 51.
     const int G = c.head_size / 32, terms = icx::attention_terms(a.dtype);
-    const size_t tokens = (size_t)a.table_width * c.page_size;
+    const size_t cus = (size_t)icx::num_cus(), width = (size_t)a.table_width * c.page_size;
+    const size_t tokens = a.window > 0 ? std::min(width, (size_t)a.window + a.max_rows) : width;
     size_t tiles = 0;
-    p.tile_waves = 4;
-    for (int waves : {8, 4}) {
-        if (!many || (waves == 8 && (tokens < 4096 || !icx::attention_wide(G, terms)))) continue;
-        const size_t tile = 16 * waves * (size_t)icx::attention_wave_tiles(G, terms);
-        tiles = std::min((size_t)a.batch * icx::cdiv(most, tile), icx::cdiv((size_t)a.rows * group, tile) + a.batch);
+    const auto cut = [&](int waves, int each) {
+        const size_t tile = 16 * (size_t)waves * each;
         p.tile_waves = waves;
-        if (c.kv_heads * icx::cdiv((size_t)a.rows * group, tile) >= (size_t)icx::num_cus()) break;
-    }
-    const size_t full = many ? c.kv_heads * tiles : heads * p.row_tiles;
-    // Shares, to fill the CUs.  For few rows with up to 3 blocks of them a CU: against 8 a CU, 46.2 us for 54.6 at 8
-    // sequences of 32768 tokens (4 bits, 32 heads over 8 of 128), 23.8 for 36.3 at 4 of 16384, 28.6 for 33.7 at 32
-    // of 4096; against 1, 70.1, 25.0 and 35.6.
-    const size_t want = (many ? (size_t)icx::num_cus() * 8 / p.tile_waves : (size_t)icx::num_cus() * 3) / std::max<size_t>(full, 1);
-    p.splits = (int)std::max<size_t>(1, std::min({want, icx::cdiv(tokens, 256), (size_t)kMaxSplits}));
+        p.wave_tiles = each;
+        tiles = std::min((size_t)a.batch * icx::cdiv(most, tile), icx::cdiv((size_t)a.rows * group, tile) + a.batch);
+        return c.kv_heads * icx::cdiv((size_t)a.rows * group, tile);
+    };
+    const size_t most_shares = std::max<size_t>(1, many ? tokens / 256 : icx::cdiv(tokens, 256));
+    const bool wide = many && tokens >= 4096 && icx::attention_wide(G, terms) && cut(8, 2) >= 2 * cus;
+    if (!wide && (icx::attention_wave_tiles(G, terms) == 1 || cut(4, 2) * most_shares < 2 * cus)) cut(4, 1);
+    const size_t full = std::max<size_t>(1, many ? c.kv_heads * tiles : heads * p.row_tiles);
+    // Shares, to fill the CUs: for many rows up to 2 blocks a CU, rounded up for small ones (12 heads of 64, 512
+    // rows over 2048 tokens 22.4 against 38.5 with one share).  For few rows up to 3 blocks: against 8 a CU, 46.2 us for
+    // 54.6 at 8 sequences of 32768 tokens (4 bits, 32 heads over 8 of 128), 23.8 for 36.3 at 4 of 16384, 28.6 for 33.7
+    // at 32 of 4096; against 1, 70.1, 25.0 and 35.6.
+    const size_t want = !many ? cus * 3 / full : p.wave_tiles == 1 ? icx::cdiv(cus * 2, full) : cus * 2 / full;
+    p.splits = (int)std::max<size_t>(1, std::min({want, most_shares, (size_t)kMaxSplits}));
     p.few = heads * p.row_tiles * p.splits;
     p.many = c.kv_heads * tiles * p.splits;
     const size_t rows = (size_t)a.rows * a.q_heads;
@@ -211,6 +222,7 @@ extern "C" int icx_kv_cache_attention(icx_stream_t stream, const icx_kv_cache* c
     a.row_tiles = p.row_tiles;
     a.few_rows = p.few_rows;
     a.tile_waves = p.tile_waves;
+    a.wave_tiles = p.wave_tiles;
     // (exact below 2^26 chunks: the remainder of 2^32 / 64 chunks at most is then worth less than one)
     a.chunks_inverse = a.l.chunks == 1 ? 0u : (uint32_t)((0x100000000ull + a.l.chunks - 1) / a.l.chunks);
     a.splits = p.splits;

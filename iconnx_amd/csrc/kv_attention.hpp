@@ -24,7 +24,7 @@ struct AttnArgs {
     const float* slopes;
     int row_tiles, splits;
     uint32_t chunks_inverse;  // ceil(2^32 / chunks of a page), 0 for one: chunk / chunks by a multiplication
-    int tile_waves;  // of a block of kv_attention_tiles_kernel
+    int tile_waves, wave_tiles;  // of a block of kv_attention_tiles_kernel: its waves, and a wave's tiles of 16 rows
     int few_rows;  // sequences of at most as many (rows times group) go to kv_attention_rows_kernel
     float* part;   // [splits][rows_total * heads_q][D] sums of exp(s - m) v
     float2* ml;    // [splits][rows_total * heads_q] (m, in powers of two; sum of exp)
@@ -49,14 +49,15 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
 // bfloat16 numbers that a query is taken apart into, and a probability is held in.
 constexpr int attention_terms(int dtype) { return dtype == ICX_BF16 ? 1 : dtype == ICX_F16 ? 2 : 3; }
 
-// Tiles of 16 rows of a wave of kv_attention_tiles_kernel: two while their queries and sums about fit the
-// registers.  (Heads of 256 in bfloat16 then keep 32 of them in memory, and are faster all the same: 2 times
-// 4096 rows over 8192 tokens 997 us for 1158 with one tile; float16 heads of 128, 5 in memory, 809 for 907.)
-constexpr int attention_wave_tiles(int G, int terms) { return G * terms >= 12 ? 1 : 2; }
-// Its blocks are of 4 waves, or for bfloat16 heads of up to 128 of 8.  (LDS holds no more of two steps.  float16
-// and float32 gain nothing from 8: 16384 rows over as many tokens 3710 us for 3503, and 5377 for 5501, 2 times
-// 4096 over 8192 981 for 853, and 1222 for 1190.)
-constexpr bool attention_wide(int G, int terms) { return G <= 4 && terms == 1; }
+// Tiles of 16 rows of a wave of kv_attention_tiles_kernel, at most: two while their queries and sums about fit
+// the registers.  (Heads of 256 in bfloat16 then keep 32 of them in memory, and are faster all the same: 2 times
+// 4096 rows over 8192 tokens 997 us for 1158 with one tile; float16 heads of 128, 5 in memory, 809 for 907.)  Heads
+// of up to 64 are as fast with one, and faster where there are few rows.
+constexpr int attention_wave_tiles(int G, int terms) { return G <= 2 || G * terms >= 12 ? 1 : 2; }
+// Its blocks are of 4 waves, or for bfloat16 heads of 64 to 128 of 8, of two tiles.  (LDS holds no more of two steps.
+// float16 and float32 gain nothing from 8: 16384 rows over as many tokens 3710 us for 3503, and 5377 for 5501, 2
+// times 4096 over 8192 981 for 853, and 1222 for 1190; heads of 32 lose: 8192 over 8192 146 for 120.)
+constexpr bool attention_wide(int G, int terms) { return G >= 2 && G <= 4 && terms == 1; }
 
 void launch_attention_bf16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);
 void launch_attention_f16(int bits, unsigned few, unsigned many, hipStream_t s, const AttnArgs& a);

@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(64 * kWaves, rows_kernel_waves(BITS, TERMS, G)
 }
 
 // ---- many rows ------------------------------------------------------------------------------------
-// One block: 32 rows a wave (16 where the queries' terms would not leave the registers for more) of one
+// One block: 32 or 16 rows a wave (icx::attention_wave_tiles, and the host's rule on how many there are) of one
 // cached head of one sequence, one share of its tokens.
 // The waves decode a step of tokens together, a chunk of 16 each, into LDS as the bfloat16 operands of
 // both products, in the order that their lanes read them back (16 bytes a lane, in lane order, so
@@ -427,9 +427,9 @@ __global__ void __launch_bounds__(64 * kWaves, rows_kernel_waves(BITS, TERMS, G)
 // A NaN of a value must not meet a weight of zero in the product.  The decoder writes zeros in its
 // place and notes it; steps with such a note, which are rare, add NaN by hand to the rows that see it.
 
-template <int BITS, int TERMS, int G, int W, typename T>
+template <int BITS, int TERMS, int G, int W, int NQ, typename T>
 __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kernel(AttnArgs a) {
-    constexpr int NQ = icx::attention_wave_tiles(G, TERMS), C = 4;  // tiles of 16 rows a wave; chunks worked on at once
+    constexpr int C = 4;  // chunks worked on at once
     constexpr int kTileRows = 16 * NQ * W;
     constexpr int kKeys = C * G * 1024;
     constexpr bool kAhead = NQ == 1 || (G <= 4 ? G * (TERMS + 2) <= 12 : G <= 6);  // (else it would not fit them)
@@ -803,13 +803,21 @@ void launch_heads(unsigned few, unsigned many, hipStream_t s, const AttnArgs& a)
         const size_t lds = kWaves * held * (32 * G + 4) * 4 + kWaves * 16 * 8;
         kv_attention_rows_kernel<BITS, TERMS, G, T><<<few, 64 * kWaves, lds, s>>>(a);
     }
+    if (!many) return;
+    constexpr int NQ = icx::attention_wave_tiles(G, TERMS);
     if constexpr (icx::attention_wide(G, TERMS)) {
-        if (many && a.tile_waves == 8) {
-            kv_attention_tiles_kernel<BITS, TERMS, G, 8, T><<<many, 512, 0, s>>>(a);
+        if (a.tile_waves == 8) {
+            kv_attention_tiles_kernel<BITS, TERMS, G, 8, 2, T><<<many, 512, 0, s>>>(a);
             return;
         }
     }
-    if (many) kv_attention_tiles_kernel<BITS, TERMS, G, 4, T><<<many, 256, 0, s>>>(a);
+    if constexpr (NQ > 1) {
+        if (a.wave_tiles == 1) {
+            kv_attention_tiles_kernel<BITS, TERMS, G, 4, 1, T><<<many, 256, 0, s>>>(a);
+            return;
+        }
+    }
+    kv_attention_tiles_kernel<BITS, TERMS, G, 4, NQ, T><<<many, 256, 0, s>>>(a);
 }
 
 template <int BITS, int TERMS, typename T>

@@ -346,6 +346,72 @@ def test_nan_and_infinity_reach_the_rows_that_see_them_alone(rows, bits, dtype):
     assert torch.equal(out, clean)
 
 
+class Many:
+    """So many heads, or so wide a table, that the tiles are the large ones; some heads are checked."""
+
+    def __init__(self, H, group, D, bits, dtype, lengths, rows, width):
+        g = torch.Generator(device="cuda").manual_seed(11)
+        self.H, self.group, self.D, self.dtype, self.lengths, self.rows = H, group, D, dtype, lengths, rows
+        pages = [-(-n // 32) for n in lengths]
+        self.cache = ops.KvCache(sum(pages), 32, H, D, bits=bits)
+        self.table = torch.zeros(len(lengths), width // 32, dtype=torch.int32)
+        self.slots, at = [], 0
+        for b, n in enumerate(pages):
+            self.table[b, :n] = torch.arange(at, at + n).flip(0)
+            j = torch.arange(lengths[b])
+            self.slots.append((self.table[b][j // 32].long() * 32 + j % 32).cuda())
+            at += n
+        self.k, self.v = ([torch.randn(n, H, D, device="cuda", generator=g) for n in lengths] for _ in range(2))
+        self.put()
+        self.q = torch.randn(sum(rows), H * group, D, device="cuda", generator=g).to(dtype)
+        self.starts = np.cumsum([0] + list(rows))
+
+    def put(self):
+        for b, s in enumerate(self.slots):
+            ops.gpu_kv_cache_write(self.cache, self.k[b], self.v[b], s)
+
+    def attend(self, **kw):
+        i32 = torch.int32
+        return ops.gpu_kv_cache_attention(self.q, self.cache, self.table.cuda(), torch.tensor(self.lengths, dtype=i32).cuda(),
+                                          q_starts=torch.tensor(self.starts, dtype=i32).cuda(), max_rows=max(self.rows), **kw)
+
+    def check(self, **kw):
+        out = self.attend(**kw)
+        held = [ops.gpu_kv_cache_read(self.cache, s) for s in self.slots]
+        slopes = kw.pop("slopes", None)
+        for h in (0, self.H // 2 - 1, self.H - 1):
+            mine = slice(h * self.group, (h + 1) * self.group)
+            want, bound = ref.attention(self.q[:, mine], [ref.f64(k[:, h:h + 1]) for k, _ in held], [ref.f64(v[:, h:h + 1]) for _, v in held],
+                                        self.lengths, self.starts, self.D ** -0.5, terms=TERMS[self.dtype], dtype=self.dtype,
+                                        slopes=None if slopes is None else ref.f64(slopes[mine]), **kw)
+            err = np.abs(ref.f64(out[:, mine]) - want)
+            assert not np.isnan(err).any() and (err <= bound).all(), "head %d off by %g of %g" % (h, err.max(), bound[err == err.max()][0])
+        return out
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("H,group,D,lengths,rows,width", [
+    (8, 2, 96, [300, 150, 40], [130, 70, 3], 16384), (8, 2, 128, [300, 150, 40], [130, 70, 33], 16384),  # shares, most of them empty
+    (4, 3, 256, [290, 61], [100, 61], 32768), (180, 1, 96, [300], [270], 320), (180, 1, 128, [300], [270], 320),  # one share
+    (180, 1, 224, [200, 140], [200, 140], 224), (200, 1, 64, [300, 30], [200, 30], 320),
+    (256, 1, 64, [400, 100], [300, 20], 4096), (256, 1, 96, [400, 100], [300, 20], 4096), (180, 2, 128, [400], [300], 4096)])  # 8 waves
+def test_large_tiles(H, group, D, lengths, rows, width, bits, dtype):
+    m = Many(H, group, D, bits, dtype, lengths, rows, width)
+    clean = m.check()
+    m.check(window=70, softcap=20.0, slopes=torch.exp2(-torch.arange(1, H * group + 1).float() % 8).cuda())
+    if bits == 4:
+        m.check(causal=False)
+    # a value that is not finite, in the first sequence's third token from the end
+    m.v[0][-3, H - 1, 33] = float("nan")
+    m.put()
+    out, end = m.attend(), rows[0]
+    last = slice((H - 1) * group, H * group)
+    assert torch.isnan(out[end - 3:end, last, 32:64]).all()
+    out[end - 3:end, last, 32:64] = clean[end - 3:end, last, 32:64]
+    assert torch.equal(out, clean)
+
+
 @pytest.mark.parametrize("rows", [None, [3, 40]])
 def test_pages_outside_the_cache_are_not_seen(rows):
     f = Filled([100, 90], 2, 64, 16, 4)
