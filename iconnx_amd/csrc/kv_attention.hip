@@ -88,7 +88,7 @@ void launch_join(hipStream_t s, const AttnArgs& a) {
 
 // How the call is cut: tiles of rows and shares of the tokens.
 struct Plan {
-    int row_tiles, few_rows, splits, tile_waves, wave_tiles;
+    int row_tiles, few_rows, splits, tile_waves = 4, wave_tiles = 1;
     size_t few, many, part_bytes, ml_bytes;  // blocks of either kernel, workspace
 };
 constexpr size_t kFewRows = 32;
@@ -125,8 +125,10 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
         return c.kv_heads * icx::cdiv((size_t)a.rows * group, tile);
     };
     const size_t most_shares = std::max<size_t>(1, many ? tokens / 256 : icx::cdiv(tokens, 256));
-    const bool wide = many && tokens >= 4096 && icx::attention_wide(G, terms) && cut(8, 2) >= 2 * cus;
-    if (!wide && (icx::attention_wave_tiles(G, terms) == 1 || cut(4, 2) * most_shares < 2 * cus)) cut(4, 1);
+    if (many) {
+        const bool wide = tokens >= 4096 && icx::attention_wide(G, terms) && cut(8, 2) >= 2 * cus;
+        if (!wide && (icx::attention_wave_tiles(G, terms) == 1 || cut(4, 2) * most_shares < 2 * cus)) cut(4, 1);
+    }
     const size_t full = std::max<size_t>(1, many ? c.kv_heads * tiles : heads * p.row_tiles);
     // Shares, to fill the CUs: for many rows up to 2 blocks a CU, rounded up for small ones (12 heads of 64, 512
     // rows over 2048 tokens 22.4 against 38.5 with one share).  For few rows up to 3 blocks: against 8 a CU, 46.2 us for
