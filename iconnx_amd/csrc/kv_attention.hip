@@ -55,8 +55,11 @@ __global__ void __launch_bounds__(64 * kJoinWaves) kv_attention_join_kernel(Attn
     for (int s = 0; s < a.splits; s += N) {
         const int mine = s + first;
         const float w = __shfl(f, min(mine, 63), 64);
-        // (a share that saw no token has the weight 0, and may have left nothing to read)
-        if (mine < a.splits && d < D && w != 0.0f) sum += w * *reinterpret_cast<const f32x4*>(a.part + (mine * all + at) * D + d);
+        if (mine >= a.splits || d >= D) continue;
+        const f32x4 part = *reinterpret_cast<const f32x4*>(a.part + (mine * all + at) * D + d);
+        // (a weight that is no number any more takes out what its share summed, but not a NaN that the row sees)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += w != 0.0f || part[k] != part[k] ? w * part[k] : 0.0f;
     }
 #pragma unroll
     for (int off = L; off < 64; off <<= 1)

@@ -55,6 +55,17 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[TER
         }
 }
 
+// The same of a query.  One that is infinite counts as NaN, which its scores and their differences come to; of two
+// terms or three the second says so itself.
+template <int TERMS>
+__device__ __forceinline__ void split_query(float (&v)[8], bf16x8 (&t)[TERMS]) {
+    if constexpr (TERMS == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += v[e] * 0.0f;
+    }
+    split_terms<TERMS>(v, t);
+}
+
 // cap tanh(x), x given in units of log2(e) / 2: through exp2, and in float32 (TERMS 3) by its series near 0,
 // where that form's error, 2^-22 of the cap, is not below a score's own any more.  (The other types' caps end at
 // 1024, where the error is half of float16's rounding of the weight; with the series in them too, for larger
@@ -236,7 +247,7 @@ __global__ void __launch_bounds__(64 * kWaves, rows_kernel_waves(BITS, TERMS, G)
         for (int i = 0; i < G; ++i) {
             float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (row_there) icx::load_f32(qp + 8 * i, v);
-            split_terms<TERMS>(v, qf[i]);
+            split_query<TERMS>(v, qf[i]);
         }
     }
 
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(64 * W, G > 4 ? 1 : 2) kv_attention_tiles_kern
             icx::load_f32(qp[t] + 8 * i, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= sign;
-            split_terms<TERMS>(v, qf[t][i]);
+            split_query<TERMS>(v, qf[t][i]);
         }
     if (from < to) decode(0);
     __syncthreads();

@@ -409,7 +409,8 @@ int icx_kv_cache_read(icx_stream_t stream, const icx_kv_cache* cache, const void
  *   out = softmax_j(cap(scale q.k_j) + slopes[h] (j - p)) v_j  over  j <= p (causal) and j > p - window
  * (window 0: no limit), cap(s) = softcap tanh(s / softcap) (softcap 0 or infinite: none; otherwise up
  * to 1024, in ICX_F32 2^64), slopes [q_heads] f32 or
- * NULL.  A row that sees no token is zero; tokens in a page outside the cache are not seen.  Rows of
+ * NULL.  A row that sees no token is zero; tokens in a page outside the cache are not seen.  A weight stands in
+ * the f32 sums as up to 256: 256 times what a row's values add up to has to stay below 2^128.  Rows of
  * out that belong to no sequence are left as they were. */
 typedef struct icx_kv_attention {
     const void* q;

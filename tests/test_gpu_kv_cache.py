@@ -346,6 +346,27 @@ def test_nan_and_infinity_reach_the_rows_that_see_them_alone(rows, bits, dtype):
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [2, 40])
+def test_what_is_not_finite_far_below_the_largest_score(rows, dtype):
+    """A token whose weight vanishes beside another share's still makes the rows that see it NaN; a query that is
+    infinite makes its row NaN, though every score of it be minus infinity."""
+    f = Filled([3000], 1, 64, 16, 8)
+    k, v = torch.randn(3000, 1, 64) * 0.1, torch.randn(3000, 1, 64)
+    k[:, 0, 0] = torch.where(torch.arange(3000) < 1500, -400.0, -1.0)
+    v[7, 0, 40] = float("inf")
+    f.put(0, k, v)
+    q = query(rows, 1, 64, dtype)
+    q[:, 0, 0] = 30.0
+    out = f.attend(q, [rows])
+    assert torch.isnan(out[:, :, 32:]).all() and torch.isfinite(out[:, :, :32]).all()
+    v[7, 0, 40] = 0.0
+    f.put(0, k, v)
+    q[1, 0, 0] = float("inf")
+    out = f.attend(q, [rows])
+    assert torch.isnan(out[1]).all() and torch.isfinite(out[0]).all() and torch.isfinite(out[2:]).all()
+
+
 class Many:
     """So many heads, or so wide a table, that the tiles are the large ones; some heads are checked."""
 
