@@ -198,10 +198,11 @@ __device__ __forceinline__ float finish(int acc, float xs, float ws, float bias)
 // ---- few tokens ---------------------------------------------------------------------------------
 // 16 tokens by 16 channels a block, K split over its eight waves (integers: the same sum in any order).
 // What such a product costs is the walk of the weight, so its loads come first and many at a time: a
-// wave's share of K in groups of U steps of 64, all of a group's fragments asked for before the first is
-// used.  q's fragments come from L2, or with QUANT from LDS, where every block puts all tokens' bytes
-// after asking for its first weights: it quantizes them itself (the same work in every block, under
-// the latency of the weight's walk, in place of a launch before this one), a wave a row.
+// wave's share of K in groups of U steps of 64, all of a group's fragments asked for while the group
+// before it is multiplied (8192 x 4096, 9 tokens, 12.9 us for 14.2 one after another).  q's fragments
+// come from L2, or with QUANT from LDS, where every block puts all tokens' bytes after asking for its
+// weights: it quantizes them itself (the same work in every block, under the latency of the weight's
+// walk, in place of a launch before this one), a wave a row.
 constexpr int kSmallWaves = 8;
 
 template <bool QUANT, typename X, typename T>
@@ -216,12 +217,12 @@ __global__ void __launch_bounds__(64 * kSmallWaves) token_product_small_kernel(P
     const int8_t* b = g.w + (int64_t)min(n0 + lr, g.N - 1) * g.Kp + 16 * j;
     const int steps = g.Kp / 64, share = (steps + W - 1) / W;
     const int from = min(steps, wid * share), to = min(steps, from + share);
-    v4i fb[U];
-    auto load_b = [&](int s) {
+    auto load_b = [&](v4i (&fb)[U], int s) {
 #pragma unroll
         for (int u = 0; u < U; ++u) fb[u] = *reinterpret_cast<const v4i*>(b + min(s + u, steps - 1) * 64);
     };
-    load_b(from);
+    v4i f0[U];
+    load_b(f0, from);
     const int ld = g.Kp + 16;  // (rows 16 bytes further apart than whole steps: no two of 8 share banks)
     if constexpr (QUANT) {
         __builtin_amdgcn_sched_barrier(0);
@@ -233,12 +234,6 @@ __global__ void __launch_bounds__(64 * kSmallWaves) token_product_small_kernel(P
 #pragma unroll
             for (int i = 0; i < NV; ++i) raw[i] = ask_row8(row, (i * 64 + lane) * 8, K);
             uint32_t top = 0;
-#pragma unroll 1
-            for (int k = (NV * 64 + lane) * 8; k < K; k += 512) {
-                float u[8];
-                load_row8(row, k, K, u);
-                top = top8(u, top);
-            }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float u[8];
@@ -260,30 +255,43 @@ __global__ void __launch_bounds__(64 * kSmallWaves) token_product_small_kernel(P
                 take_row8(raw[i], row, (i * 64 + lane) * 8, K, u);
                 put((i * 64 + lane) * 8, u);
             }
-#pragma unroll 1
-            for (int k = (NV * 64 + lane) * 8; k < g.Kp; k += 512) {
-                float u[8];
-                load_row8(row, k, K, u);
-                put(k, u);
-            }
         }
         __syncthreads();
     }
     const int8_t* a = QUANT ? rows + min(lr, g.M - 1) * ld + 16 * j : g.q + (int64_t)min(m0 + lr, g.M - 1) * g.lda + 16 * j;
     v4i acc = {0, 0, 0, 0};
-    for (int s = from; s < to; s += U) {
-        if (s != from) load_b(s);
-        v4i fa[U];
-        if constexpr (!QUANT) {
+    auto multiply = [&](const v4i (&fa)[U], const v4i (&fb)[U], int s) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) fa[u] = *reinterpret_cast<const v4i*>(a + min(s + u, steps - 1) * 64);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // every load of the group before the first product
+        for (int u = 0; u < U; ++u)
+            if (s + u < to) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u], fb[u], acc, 0, 0, 0);
+    };
+    if constexpr (QUANT) {  // (a wave's share is one group)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (s + u >= to) break;
-            if constexpr (QUANT) fa[u] = *reinterpret_cast<const v4i*>(a + (s + u) * 64);
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u], fb[u], acc, 0, 0, 0);
+            if (from + u >= to) break;
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(a + (from + u) * 64), f0[u], acc, 0, 0, 0);
+        }
+    } else {
+        auto load_a = [&](v4i (&fa)[U], int s) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) fa[u] = *reinterpret_cast<const v4i*>(a + min(s + u, steps - 1) * 64);
+        };
+        v4i a0[U], a1[U], f1[U];
+        load_a(a0, from);
+        for (int s = from; s < to; s += 2 * U) {
+            if (s + U < to) {
+                load_b(f1, s + U);
+                load_a(a1, s + U);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(a0, f0, s);
+            if (s + U >= to) break;
+            if (s + 2 * U < to) {
+                load_b(f0, s + 2 * U);
+                load_a(a0, s + 2 * U);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(a1, f1, s + U);
         }
     }
     part[wid][lane] = acc;
@@ -665,17 +673,23 @@ Form form_of(size_t M, size_t K, size_t N) {
     if (tiles(128) <= 2 * c) return {kTile128, 128};
     return {kTile256, 256};
 }
-// Tokens that every block of the product quantizes for itself, and the LDS that they may take.
-constexpr size_t kFusedTokens = kSmallWaves, kFusedBytes = 128 * 1024;
+// Up to 8 tokens every block of the product quantizes for itself, where their values fit the registers and the
+// blocks run at once (twice as many for a short K); us with 1 (8) tokens, K x N, against quantizing them first: 4096 x
+// 4096 8.8 (10.0) / 9.9, 768 x 8192 7.4 (10.0) / 9.8, but 4096 x 5120 13.7 (16.6) / 12.0, 2048 x 8192 11.1 (12.6) / 9.8,
+// 768 x 12288 10.8 (13.6) / 9.8, 8192 x 4096, read twice, 16.8 (18.4) / 14.2.
+constexpr size_t kFusedTokens = kSmallWaves, kFusedK = 4096;
 inline size_t fused_lds(size_t M, size_t K) { return M * (padded(K) + 16); }
-inline bool fused(size_t M, size_t K) { return M <= kFusedTokens && fused_lds(M, K) <= kFusedBytes; }
+inline bool fused(size_t M, size_t K, size_t N) {
+    const size_t blocks = icx::cdiv(N, 16), c = (size_t)icx::num_cus();
+    return M <= kFusedTokens && K <= kFusedK && blocks <= (K <= 1024 ? 2 * c : c);
+}
 
 // q [M, Kp] and, behind it, the scales (Int8 tokens: rows that have to be padded).
 struct Workspace {
     size_t scale_off, total;
 };
-Workspace workspace(size_t M, size_t K, int x_dtype) {
-    if (x_dtype == ICX_I8 ? K % kAlignK == 0 : fused(M, K)) return {0, 0};
+Workspace workspace(size_t M, size_t K, size_t N, int x_dtype) {
+    if (x_dtype == ICX_I8 ? K % kAlignK == 0 : fused(M, K, N)) return {0, 0};
     const size_t q = icx::align_up(M * padded(K), 256);
     return {q, q + (x_dtype == ICX_I8 ? 0 : 4 * M)};
 }
@@ -724,8 +738,7 @@ extern "C" int icx_quantize_tokens(icx_stream_t stream, const void* x, int x_dty
 }
 
 extern "C" size_t icx_token_qlinear_workspace_size(size_t M, size_t K, size_t N, int x_dtype) {
-    (void)N;
-    return workspace(M, K, x_dtype).total;
+    return workspace(M, K, N, x_dtype).total;
 }
 
 extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* args, void* ws, size_t ws_bytes) {
@@ -753,7 +766,7 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* ar
     // (a tile's rows are reached by offsets of 32 bits)
     if (!own && !pad && (a.x_stride < 0 || a.x_stride > kMaxStride))
         ICX_FAIL(ICX_ERR_SHAPE, "%s: Int8 rows at a stride of %lld (must be up to %lld)", who, (long long)a.x_stride, (long long)kMaxStride);
-    const Workspace L = workspace(M, K, a.x_dtype);
+    const Workspace L = workspace(M, K, N, a.x_dtype);
     if ((own || pad) && L.total && (!ws || ws_bytes < L.total))
         ICX_FAIL(ICX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed (got %zu)", who, L.total, ws_bytes);
     const hipStream_t s = (hipStream_t)stream;
@@ -766,7 +779,7 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* ar
     g.M = (int)M;
     g.N = (int)N;
     g.Kp = (int)padded(K);
-    const bool few = own && fused(M, K);
+    const bool few = own && fused(M, K, N);
     const Form form = few ? Form{kTile16, 16} : form_of(M, K, N);
     g.tiles_m = (int)icx::cdiv(M, form.tile);
     g.tiles_n = (int)icx::cdiv(N, form.tile);

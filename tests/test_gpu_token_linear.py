@@ -77,7 +77,8 @@ def test_tokens_of_zeros_tiny_values_and_not_finite_ones(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 768, 768), (2, 100, 37), (7, 4096, 256), (16, 129, 65), (31, 1000, 500), (64, 512, 192),
                                    (65, 256, 129), (100, 3000, 77), (129, 640, 384), (257, 200, 300), (300, 1111, 263), (1025, 384, 520),
-                                   (2049, 128, 1000)])
+                                   (2049, 128, 1000), (3, 4096, 4096), (3, 4096, 4100), (3, 4097, 64), (5, 1024, 8192), (5, 1000, 8200),
+                                   (9, 20000, 48), (16, 8200, 40), (1, 6145, 33), (2, 131071, 20), (24, 40000, 17)])
 def test_product(M, K, N, dtype):
     x, w, ws, bias = inputs(M, K, N, dtype, seed=M + N, bias=(M + N) % 3 != 0)
     tw = ops.TokenWeight(w, ws)
