@@ -654,7 +654,9 @@ int quantize(hipStream_t s, const void* x, int dtype, size_t M, size_t K, int64_
 //    tiles, 16 x 4096 7.5 / 9.3; past c 64 x 1500 10.5 / 9.1, and of a short K nothing is left to share
 //    out (16 x 4096 4.8 / 4.1);
 //  * 64 x 64 tiles, with two groups of waves while there are at most c (200 x 4096 10.5 against 12.6 with one; past
-//    that 1024 x 1500 19.2 / 15.2, as LDS then holds one block a CU instead of three), to 3 c of them;
+//    that 1024 x 1500 19.2 / 15.2, as LDS then holds one block a CU instead of three), to 3 c of them, of a long K
+//    2.5 c (256 x 11008 23.6 / 21.3 with 128 x 128), and to 5 c where tiles of 128, one a CU, would start a second
+//    round (384 x 11008 32.5 / 40.4, at 768 values 2048 x 2304 11.8 / 14.9; at 512 x 11008, 5.4 c, 40.5 / 41.5);
 //  * 128 x 128 tiles to 2 c of them: 1024 x 4096 24.2 (8.7) against 30.8 (10.6) with 64 x 64 and 45 (15) with
 //    256 x 256; at 600 x 4096, 640 tiles of 64, 21.8 (8.0) / 22.7 (7.7);
 //  * 256 x 256 tiles: 8192 x 1500 53.8 (20.9) against 68.8 (21.7) with 128 x 128; at 2048 x 4096, 512 tiles of
@@ -669,7 +671,7 @@ Form form_of(size_t M, size_t K, size_t N) {
     const auto tiles = [&](size_t t) { return icx::cdiv(M, t) * icx::cdiv(N, t); };
     if (K >= 2048 && tiles(16) <= c) return {kTile16, 16};
     if (tiles(64) <= c) return {kTile64Shared, 64};
-    if (tiles(64) <= 3 * c) return {kTile64, 64};
+    if (tiles(64) <= (K >= 2048 ? 5 * c / 2 : 3 * c) || (tiles(128) > c && tiles(64) <= 5 * c)) return {kTile64, 64};
     if (tiles(128) <= 2 * c) return {kTile128, 128};
     return {kTile256, 256};
 }
