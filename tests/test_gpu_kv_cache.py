@@ -542,6 +542,32 @@ def test_two_streams_at_once():
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_two_captured_calls_replayed_at_once():
+    """Two graphs of calls with shares to join, replayed on two streams and beside eager calls: none meets another's
+    workspace."""
+    fs = [Filled([2500, 1700], 2, 128, 16, 4, seed=s) for s in (0, 1)]
+    q = query(2, 8, 128, torch.bfloat16)
+    want = [f.attend(q) for f in fs]
+    side, graphs, outs = [torch.cuda.Stream() for _ in fs], [], []
+    args = [(f.table.cuda(), torch.tensor(f.lengths, dtype=torch.int32).cuda()) for f in fs]
+    torch.cuda.synchronize()
+    for f, s, a in zip(fs, side, args):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(ops.gpu_kv_cache_attention(q, f.cache, *a))
+        graphs.append(g)
+    for n in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = fs[0].attend(q)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0]) and all(torch.equal(o, w) for o, w in zip(outs, want)), n
+
+
 @pytest.mark.parametrize("rows", [None, [50]])
 def test_a_cache_past_four_gigabytes(rows):
     pages, page, H, D = 1100, 1024, 8, 256
