@@ -154,15 +154,19 @@ struct Plan {
     int row_tiles, few_rows, splits, tile_waves = 4, wave_tiles = 1;
     size_t few, many, part_bytes, ml_bytes;  // blocks of either kernel, workspace
 };
-constexpr size_t kFewRows = 32;
+// Rows times group of a sequence.  Up to kFew, all of a batch go to the kernel of few rows (16 sequences of up to 8192
+// tokens, 8 bits, 32 heads over 8 of 128, 9 rows 67 us against 136, 12 95 / 113, 16 107 / 112, float16 108 / 135, but 4 of
+// 32768 125 / 107; 20 rows 110 / 115, 24 160 / 114).  In a batch with more than that, those up to kFewBeside do (20 rows:
+// 158 us with all up to 64 there).
+constexpr size_t kFew = 64, kFewBeside = 32;
 Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     Plan p;
     const size_t group = (size_t)(a.q_heads / c.kv_heads), most = (size_t)std::min(a.max_rows, a.rows) * group;
     const size_t heads = (size_t)a.batch * c.kv_heads;
-    const bool many = most > kFewRows;
+    const bool many = most > kFew;
     // Beside sequences of many rows, those of few have a kernel of their own where they may well be most of
     // the batch; else, and in a batch of one, the launch (4 us) costs more than it gives.
-    p.few_rows = many && (a.batch == 1 || (size_t)a.rows * group > 2 * kFewRows * a.batch) ? 0 : (int)kFewRows;
+    p.few_rows = !many ? (int)kFew : a.batch == 1 || (size_t)a.rows * group > 2 * kFewBeside * a.batch ? 0 : (int)kFewBeside;
     p.row_tiles = (int)icx::cdiv(std::min(most, (size_t)p.few_rows), 16);
     // Tiles of all sequences together (each may end in a part of one) and shares of the tokens that a row may see,
     // by the blocks that they make.  Decoding the tokens costs a block the same for 64, 128 or 256 rows of tiles;

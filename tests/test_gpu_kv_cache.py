@@ -247,6 +247,14 @@ def test_chunks_of_rows(Hq, Hkv, D, page, bits, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("Hq,Hkv,D,rows", [(2, 2, 64, [33, 64, 17, 1]), (6, 2, 96, [21, 16, 0, 11]), (4, 1, 256, [16, 13, 1, 5])])
+def test_up_to_four_tiles_of_rows(Hq, Hkv, D, rows, bits, dtype):
+    f = Filled([90, 64, 600, 11], Hkv, D, 16, bits)
+    f.check(query(sum(rows), Hq, D, dtype), rows, max_rows=max(rows))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kw", [dict(window=1), dict(window=20), dict(window=1000), dict(softcap=3.0), dict(softcap=30.0, window=50),
                                 dict(slopes=True), dict(slopes=True, softcap=10.0, window=33), dict(causal=False),
                                 dict(causal=False, window=40, slopes=True), dict(scale=0.5), dict(scale=-0.2), dict(scale=0.0)])
