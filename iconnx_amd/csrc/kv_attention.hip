@@ -155,8 +155,8 @@ struct Plan {
     size_t few, many, part_bytes, ml_bytes;  // blocks of either kernel, workspace
 };
 // Rows times group of a sequence.  Up to kFew, all of a batch go to the kernel of few rows (16 sequences of up to 8192
-// tokens, 8 bits, 32 heads over 8 of 128, 9 rows 67 us against 136, 12 95 / 113, 16 107 / 112, float16 108 / 135, but 4 of
-// 32768 125 / 107; 20 rows 110 / 115, 24 160 / 114).  In a batch with more than that, those up to kFewBeside do (20 rows:
+// tokens, 8 bits, 32 heads over 8 of 128, 9 rows 67 us against 136, 12 75 / 113, 16 91 / 112, float16 96 / 135; 4 of
+// 32768 107 / 107; 24 rows 160 / 114 before tiles shared an L2).  In a batch with more than that, those up to kFewBeside do (20 rows:
 // 158 us with all up to 64 there).
 constexpr size_t kFew = 64, kFewBeside = 32;
 Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
@@ -203,7 +203,7 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     // at 32 of 4096; against 1, 70.1, 25.0 and 35.6.
     const size_t want = !many ? cus * 3 / full : p.wave_tiles == 1 ? icx::cdiv(cus * 2, full) : cus * 2 / full;
     p.splits = (int)std::max<size_t>(1, std::min({want, most_shares, (size_t)kMaxSplits}));
-    p.few = heads * p.row_tiles * p.splits;
+    p.few = p.row_tiles > 1 ? icx::align_up(heads * p.splits, 8) * p.row_tiles : heads * p.row_tiles * p.splits;
     p.many = c.kv_heads * tiles * p.splits;
     const size_t rows = (size_t)a.rows * a.q_heads;
     p.part_bytes = p.splits > 1 ? icx::align_up((size_t)p.splits * rows * c.head_size * 4, 256) : 0;
