@@ -196,12 +196,23 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
         const bool wide = tokens >= 4096 && icx::attention_wide(G, terms) && cut(8, 2) >= 2 * cus;
         if (!wide && (icx::attention_wave_tiles(G, terms) == 1 || cut(4, 2) * most_shares < 2 * cus)) cut(4, 1);
     }
-    const size_t full = std::max<size_t>(1, many ? c.kv_heads * tiles : heads * p.row_tiles);
-    // Shares, to fill the CUs: for many rows up to 2 blocks a CU, rounded up for small ones (12 heads of 64, 512
-    // rows over 2048 tokens 22.4 against 38.5 with one share).  For few rows up to 3 blocks: against 8 a CU, 46.2 us for
-    // 54.6 at 8 sequences of 32768 tokens (4 bits, 32 heads over 8 of 128), 23.8 for 36.3 at 4 of 16384, 28.6 for 33.7
-    // at 32 of 4096; against 1, 70.1, 25.0 and 35.6.
-    const size_t want = !many ? cus * 3 / full : p.wave_tiles == 1 ? icx::cdiv(cus * 2, full) : cus * 2 / full;
+    // Shares, to fill the CUs.  For few rows up to 3 blocks a CU: against 8 a CU, 46.2 us for 54.6 at 8 sequences of 32768
+    // tokens (4 bits, 32 heads over 8 of 128), 23.8 for 36.3 at 4 of 16384, 28.6 for 33.7 at 32 of 4096; against 1, 70.1,
+    // 25.0 and 35.6.  For many rows by the tiles that there likely are, one row a sequence left out as another kernel's
+    // or no tile of its own: at least one for each CU and 3 in all where there are tokens to share (4 sequences of 300
+    // rows over 16384 tokens, 4 bits, 391 us for 557 with one share, but 8 of 1024 over 1024 81 and 141 with two; blocks
+    // of 8 waves are as many as they need to be); fewer tiles make up to 2 blocks a CU (512 rows and 15 of one over
+    // 16384 tokens 296 us for 501 with one share, 378 with 3), or 3 small ones (the same of 12 heads of 64, 429 with one,
+    // 136 with 8).
+    size_t want = 1;
+    if (!many) {
+        want = cus * 3 / std::max<size_t>(1, heads * p.row_tiles);
+    } else if (p.tile_waves == 4) {
+        const size_t tile = 64 * (size_t)p.wave_tiles, rows = (size_t)std::max(a.rows - a.batch, 0) * group;
+        const size_t likely = c.kv_heads * std::max<size_t>(1, std::min(tiles, icx::cdiv(rows, tile)));
+        if (likely >= cus) want = tokens >= 1280 ? icx::cdiv(3 * cus, likely) : 1;
+        else want = p.wave_tiles == 1 ? icx::cdiv(3 * cus, likely) : 2 * cus / likely;
+    }
     p.splits = (int)std::max<size_t>(1, std::min({want, most_shares, (size_t)kMaxSplits}));
     p.few = p.row_tiles > 1 ? icx::align_up(heads * p.splits, 8) * p.row_tiles : heads * p.row_tiles * p.splits;
     p.many = c.kv_heads * tiles * p.splits;
