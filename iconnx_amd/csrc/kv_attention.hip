@@ -156,8 +156,8 @@ struct Plan {
 };
 // Rows times group of a sequence.  Up to kFew, all of a batch go to the kernel of few rows (16 sequences of up to 8192
 // tokens, 8 bits, 32 heads over 8 of 128, 9 rows 67 us against 136, 12 75 / 113, 16 91 / 112, float16 96 / 135; 4 of
-// 32768 107 / 107; 24 rows 160 / 114 before tiles shared an L2).  In a batch with more than that, those up to kFewBeside do (20 rows:
-// 158 us with all up to 64 there).
+// 32768 107 / 107; 24 rows 160 / 114 before tiles shared an L2).  In a batch with more than that, those up to
+// kFewBeside do (of 20 rows 114 us, 158 with all up to 64 there).
 constexpr size_t kFew = 64, kFewBeside = 32;
 Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     Plan p;
@@ -199,19 +199,19 @@ Plan plan_of(const icx_kv_cache& c, const icx_kv_attention& a) {
     // Shares, to fill the CUs.  For few rows up to 3 blocks a CU: against 8 a CU, 46.2 us for 54.6 at 8 sequences of 32768
     // tokens (4 bits, 32 heads over 8 of 128), 23.8 for 36.3 at 4 of 16384, 28.6 for 33.7 at 32 of 4096; against 1, 70.1,
     // 25.0 and 35.6.  For many rows by the tiles that there likely are, one row a sequence left out as another kernel's
-    // or no tile of its own: at least one for each CU and 3 in all where there are tokens to share (4 sequences of 300
-    // rows over 16384 tokens, 4 bits, 391 us for 557 with one share, but 8 of 1024 over 1024 81 and 141 with two; blocks
-    // of 8 waves are as many as they need to be); fewer tiles make up to 2 blocks a CU (512 rows and 15 of one over
-    // 16384 tokens 296 us for 501 with one share, 378 with 3), or 3 small ones (the same of 12 heads of 64, 429 with one,
-    // 136 with 8).
+    // or no tile of its own: 3 blocks a CU or more where there are tiles for each CU or tiles are small (4 sequences of
+    // 300 rows over 16384 tokens, 4 bits, 391 us for 557 with one share; 512 rows and 15 of one over as many, 12 heads of
+    // 64, 136 for 429), up to 2 else (the same of 32 heads over 8 of 128 296 for 501, but 378 with 3 shares), up to one
+    // where the tokens are few (of 1024 tokens 2 heads of 256, 32 sequences of up to 128 rows 54 us, 75 with 4 shares; 8 of
+    // 1024, 32 heads over 8 of 128, 81, 141 with 2).  Blocks of 8 waves are as many as they need to be.
     size_t want = 1;
     if (!many) {
         want = cus * 3 / std::max<size_t>(1, heads * p.row_tiles);
     } else if (p.tile_waves == 4) {
         const size_t tile = 64 * (size_t)p.wave_tiles, rows = (size_t)std::max(a.rows - a.batch, 0) * group;
         const size_t likely = c.kv_heads * std::max<size_t>(1, std::min(tiles, icx::cdiv(rows, tile)));
-        if (likely >= cus) want = tokens >= 1280 ? icx::cdiv(3 * cus, likely) : 1;
-        else want = p.wave_tiles == 1 ? icx::cdiv(3 * cus, likely) : 2 * cus / likely;
+        if (tokens < 1280) want = cus / likely;
+        else want = likely >= cus || p.wave_tiles == 1 ? icx::cdiv(3 * cus, likely) : 2 * cus / likely;
     }
     p.splits = (int)std::max<size_t>(1, std::min({want, most_shares, (size_t)kMaxSplits}));
     p.few = p.row_tiles > 1 ? icx::align_up(heads * p.splits, 8) * p.row_tiles : heads * p.row_tiles * p.splits;

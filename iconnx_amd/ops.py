@@ -677,7 +677,7 @@ def gpu_quantize_tokens(x):
     q = _empty(shape[:-1] + (Kp,), dtype=_I8, device=dev)
     scale = _empty(shape[:-1], dtype=_F32, device=dev)
     check(lib().icx_quantize_tokens(_stream(), x.data_ptr(), code, M, K, ld, q.data_ptr(), Kp, scale.data_ptr()))
-    return (q if Kp == K else q[..., :K]), scale
+    return (q if Kp == K else q.narrow(-1, 0, K)), scale
 
 
 # (arguments by struct: packing thirteen values costs a fifth of converting them one by one)
@@ -822,7 +822,7 @@ def gpu_kv_cache_read(cache, slots, dtype=torch.float32):
     n, dev = slots.shape[0], slots.device
     shape = (n,) + cache._heads
     k = _empty(shape, dtype=dtype, device=dev)
-    v = _empty(shape, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     check(lib().icx_kv_cache_read(_stream(), cache, slots.data_ptr(), sc, n, k.data_ptr(), v.data_ptr(), code))
     return k, v
 
@@ -863,7 +863,10 @@ def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_row
     if out is not None and (out.dtype != q.dtype or out.shape != shape or out.stride(2) != 1):
         raise IconnxError(ERR_SHAPE, "%s: out must be a %s %s with dense heads" % (who, _name(q.dtype), list(shape)))
     here = _here()
-    _on_device(who, here, q, page_table, lengths, q_starts, slopes, out, None if cache._device == here else cache.data)
+    if q.get_device() != here or page_table.get_device() != here or lengths.get_device() != here or cache._device != here:
+        _on_device(who, here, q, page_table, lengths, cache.data)
+    if q_starts is not None or slopes is not None or out is not None:
+        _on_device(who, here, q_starts, slopes, out)
     qr, qh, one = q.stride()
     if one != 1:
         q = q.contiguous()
@@ -875,9 +878,8 @@ def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_row
     lengths = _dense(lengths)
     if q_starts is not None:
         q_starts = _dense(q_starts)
-    dev = q.device
     if out is None:
-        out = q.new_empty((rows, heads, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     orow, oh, _ = out.stride()
     if max_rows is None:
         max_rows = 1 if q_starts is None else rows
@@ -887,7 +889,7 @@ def gpu_kv_cache_attention(q, cache, page_table, lengths, q_starts=None, max_row
         max_rows, ts[1], D ** -0.5 if scale is None else scale, softcap, window, 1 if causal else 0)
     L = lib()
     nws = L.icx_kv_cache_attention_workspace_size(cache, args)
-    ws = _empty(nws, dtype=_U8, device=dev) if nws else None
+    ws = _empty(nws, dtype=_U8, device=q.device) if nws else None
     check(L.icx_kv_cache_attention(_stream(), cache, args, None if ws is None else ws.data_ptr(), nws))
     return out
 
