@@ -634,14 +634,17 @@ __global__ void __launch_bounds__(kThreads) token_pad_kernel(const int8_t* q, in
     for (int k = threadIdx.x; k < Kp; k += kThreads) out[m * Kp + k] = k < K ? q[m * ld + k] : (int8_t)0;
 }
 
+// (of 256 threads: a launch has less than 2^32)
+constexpr size_t kMaxBlocks = 0xffffff;
 int quantize(hipStream_t s, const void* x, int dtype, size_t M, size_t K, int64_t ldx, int8_t* q, size_t ldq, size_t fill,
              float* scale) {
     const bool vec = ldq % 8 == 0 && fill % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
     const bool wide = K > 1024;
-    const unsigned blocks = (unsigned)(wide ? M : icx::cdiv(M, kThreads / 64));
+    const size_t blocks = wide ? M : icx::cdiv(M, kThreads / 64);
+    if (blocks > kMaxBlocks) ICX_FAIL(ICX_ERR_UNSUPPORTED, "QuantizeTokens: %zu tokens a call are too many", M);
     return icx::with_float_type(dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        auto launch = [&](auto kernel) { kernel<<<blocks, kThreads, 0, s>>>((const T*)x, M, (int)K, ldx, q, ldq, (int)fill, scale); };
+        auto launch = [&](auto kernel) { kernel<<<(unsigned)blocks, kThreads, 0, s>>>((const T*)x, M, (int)K, ldx, q, ldq, (int)fill, scale); };
         if (wide) vec ? launch(token_quantize_kernel<4, T, true>) : launch(token_quantize_kernel<4, T, false>);
         else vec ? launch(token_quantize_kernel<1, T, true>) : launch(token_quantize_kernel<1, T, false>);
         ICX_LAUNCH_CHECK("token_quantize_kernel");
@@ -811,6 +814,7 @@ extern "C" int icx_token_qlinear(icx_stream_t stream, const icx_token_linear* ar
         g.lda = (int64_t)padded(K);
         g.xs = sc;
     } else if (pad) {
+        if (M > kMaxBlocks) ICX_FAIL(ICX_ERR_UNSUPPORTED, "%s: %zu tokens a call are too many", who, M);
         token_pad_kernel<<<(unsigned)M, kThreads, 0, s>>>((const int8_t*)a.x, a.x_stride, (int)K, (int)padded(K), (int8_t*)ws);
         ICX_LAUNCH_CHECK("token_pad_kernel");
         g.q = (const int8_t*)ws;

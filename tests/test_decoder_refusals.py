@@ -108,4 +108,7 @@ def test_products_that_are_refused(L):
     assert L.icx_quantize_tokens(None, PTR, F32, 1, 0, 64, PTR, 64, PTR) == SHAPE
     assert L.icx_quantize_tokens(None, None, F32, 1, 64, 64, PTR, 64, PTR) == BAD
     assert L.icx_quantize_tokens(None, PTR, F32, 1, 64, 64, PTR, 63, PTR) == SHAPE
+    assert L.icx_quantize_tokens(None, PTR, F32, 1 << 24, 2048, 2048, PTR, 2048, PTR) == UNSUPPORTED
+    assert L.icx_quantize_tokens(None, PTR, F32, 1 << 26, 64, 64, PTR, 64, PTR) == UNSUPPORTED
+    assert run(xt=I8, xs=PTR, K=100, M=1 << 24, work=PTR, n=1 << 40) == UNSUPPORTED
     assert L.icx_quantize_tokens(None, None, F32, 0, 64, 64, None, 64, None) == 0
