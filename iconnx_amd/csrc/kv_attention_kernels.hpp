@@ -90,13 +90,16 @@ struct Tile {
 };
 
 // N dwords that stand at a multiple of 4 bytes, of 8 where N is even and of 16 where 4 divides it.
-template <int N>
+// PAST: not to be kept in the caches.
+template <bool PAST, int N>
 __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&d)[N]) {
     constexpr int W = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
     typedef uint32_t vec __attribute__((ext_vector_type(W)));
 #pragma unroll
     for (int i = 0; i < N / W; ++i) {
-        const vec w = reinterpret_cast<const vec*>(p)[i];
+        vec w;
+        if constexpr (PAST) w = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p) + i);
+        else w = reinterpret_cast<const vec*>(p)[i];
 #pragma unroll
         for (int e = 0; e < W; ++e) d[W * i + e] = w[e];
     }
@@ -108,12 +111,12 @@ __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&d)[N]) 
 template <int G>
 constexpr bool kSameByte = G % 4 == 0 || G <= 2;
 
-template <int BITS, int G>
+template <int BITS, int G, bool PAST = false>
 __device__ __forceinline__ void load_chunk(const uint8_t* c, int lane, Tile<BITS, G>& t, int n) {
     const int lr = lane & 15, j = lane >> 4;
-    load_dwords(c + (lr * 4 + j) * G * BITS, t.k[n]);
-    load_dwords(c + icx::kv_codes(G, BITS) + (j * 16 + lr) * G * BITS, t.v[n]);
-    load_dwords(c + icx::kv_value_scales(G, BITS) + j * 4 * G, t.vs[n]);
+    load_dwords<PAST>(c + (lr * 4 + j) * G * BITS, t.k[n]);
+    load_dwords<PAST>(c + icx::kv_codes(G, BITS) + (j * 16 + lr) * G * BITS, t.v[n]);
+    load_dwords<false>(c + icx::kv_value_scales(G, BITS) + j * 4 * G, t.vs[n]);
     const uint8_t* sp = c + icx::kv_key_scales(G, BITS) + lr * G;
     const int at = j * G >> 2;
     if constexpr (G == 8) {
@@ -198,7 +201,8 @@ __device__ __forceinline__ const uint8_t* chunk_at(const AttnArgs& a, const uint
 constexpr int kWaves = 4;
 
 // Waves a SIMD that its registers are kept to: sums, queries, two tiles of codes, and about 55 more.  (64
-// sequences of up to 8192 tokens, 4 bits, heads of 128: 104 us with the two that the compiler takes, 88 with three.)
+// sequences of up to 8192 tokens, 4 bits, heads of 128: 104 us with the two that the compiler takes, 88 with three, codes in the
+// caches.)
 constexpr int rows_kernel_waves(int bits, int terms, int G) {
     const int registers = 8 * G + 4 * G * terms + 4 * (G * bits / 2 + G + 1) + 55;
     return registers <= 160 ? 3 : registers <= 225 ? 2 : 1;
@@ -272,10 +276,15 @@ __global__ void __launch_bounds__(64 * kWaves, rows_kernel_waves(BITS, TERMS, G)
         const int chunk = (tile0 + min(i, to - 1)) * 2;
         return Next{{page_of_chunk(a, table, chunk), page_of_chunk(a, table, chunk + 1)}};
     };
+    // A call reads a code once, and by the next one most caches have passed through memory: where a lane's codes are
+    // one load of 16 bytes, an instruction's whole lines, they are read past the caches (64 sequences of up to 8192 tokens,
+    // 4 bits, heads of 128, 83 us for 92; heads of 64 in 8 bits 77 for 85; 8 bits of 128, two loads a lane that share
+    // lines, 167 for 158, and heads of 96 in 4 bits 43 for 40, are left).
+    constexpr bool kPast = G * BITS == 16;
     auto fetch = [&](Tile<BITS, G>& t, int i, const Next& n) {
         const int chunk = (tile0 + min(i, to - 1)) * 2;
-        load_chunk<BITS, G>(chunk_at(a, head, n.page[0], chunk), lane, t, 0);
-        load_chunk<BITS, G>(chunk_at(a, head, n.page[1], chunk + 1), lane, t, 1);
+        load_chunk<BITS, G, kPast>(chunk_at(a, head, n.page[0], chunk), lane, t, 0);
+        load_chunk<BITS, G, kPast>(chunk_at(a, head, n.page[1], chunk + 1), lane, t, 1);
     };
     auto work = [&](Tile<BITS, G>& t, int i, const Next& pl) {
         const int t0 = (tile0 + i) * 32;

@@ -601,6 +601,21 @@ def test_a_cache_past_four_gigabytes(rows):
     assert torch.equal(run(cache, pages - 2), run(small, 0))
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_read_larger_than_the_gpus_caches(bits):
+    H, D, n = 16, 128, 40000
+    cache = ops.KvCache(n // 16 + 3, 16, H, D, bits=bits)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(n, H, D, device="cuda", generator=g) for _ in range(2))
+    slots = torch.arange(n, device="cuda") + 21
+    slots[5000:5003] = -1
+    ops.gpu_kv_cache_write(cache, k, v, slots)
+    rk, rv = ops.gpu_kv_cache_read(cache, slots)
+    for a in range(0, n, 1000):
+        sk, sv = ops.gpu_kv_cache_read(cache, slots[a:a + 1000])
+        assert torch.equal(rk[a:a + 1000], sk) and torch.equal(rv[a:a + 1000], sv)
+
+
 def test_a_cache_keeps_its_memory():
     cache = ops.KvCache(4, 16, 2, 64)
     with pytest.raises(AttributeError):
